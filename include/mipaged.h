@@ -14,6 +14,8 @@
  *                           prefixes and themselves, causal, reading K/V pages in place.
  *   5. Layer elementwise  : residual add + RMS norm, and SiLU(gate) * up.
  *   6. Small linear       : linear layers of a decode step with norm, bias, residual or gating fused.
+ *   7. Drafted trees      : a step of speculative decoding: the nodes' places and ancestors, attention
+ *                           of a tree's nodes over the cache, verification, the accepted rows' move.
  *
  * Pool layout (one layer; identical to the reference pool
  * engine/kv_cache.py:426-428, `k, v: [num_layers, num_blocks + 1, num_kv_heads,
@@ -422,6 +424,81 @@ int mip_decode_prepare(int32_t* rows, int64_t row_stride, const int64_t* journal
  */
 int mip_rope_tables(void* cos, void* sin, const int64_t* positions, int32_t n_tokens, int32_t head_dim, float theta,
                     int32_t dtype, void* stream);
+
+/*
+ * Drafted trees (speculative decoding; no reference counterpart: the reference decodes one token a
+ * step). Sequence s has c = ctx_start[s] cached tokens and a tree of n = cu_q[s + 1] - cu_q[s] nodes, its
+ * packed rows r = cu_q[s] + i. Node 0 is the sequence's last token, which is not cached yet; every other
+ * node is a drafted token that continues its parent. Node i's key and value are cache index c + i (append
+ * them first); its rotary position is c + its depth. max_q_len must be >= every n (nodes from max_q_len
+ * on are passed by) and sizes the grids; rows that belong to no sequence are not written.
+ *
+ * mip_paged_tree: attention of the nodes,
+ *
+ *   out[r, h, :] = softmax_j( scale * q[r, h, :] . K_s[j, :] ) @ V_s[j, :]
+ *       over j < c, and j = c + e where bit e % 64 of mask[r * mask_stride + e / 64] is set, e < n,
+ *   K_s[j] = k_cache row (block_tables[s * bt_stride + j / block_size], h / group, j % block_size)
+ *
+ * A row that sees no key becomes zeros, a key that a row does not see has no influence on it whatever its
+ * bytes are, and a key whose block id lies outside the pool is seen by no row. Keys past
+ * max_blocks_per_seq * block_size are never read. mask_words >= ceil(max_q_len / 64). scale > 0.
+ * Scores, sums and products accumulate in fp32; 16-bit types at head_dim 64 / 128 (q rows 16-byte, output
+ * rows 8-byte aligned, at most 1024 sequences) run on the matrix cores, with the softmax weights rounded
+ * to fp16 as in mip_paged_prefill. Other calls take one workgroup per (node, query head): any type, head_dim a
+ * power of two in 8 .. 256 (others: MIP_EUNSUPPORTED), element alignment.
+ * The workspace holds mip_paged_tree_workspace(..) bytes, 256-byte aligned, asked with the same device
+ * current; contents and reuse as for mip_paged_decode.
+ */
+size_t mip_paged_tree_workspace(int32_t num_seqs, int32_t max_q_len, int32_t num_heads, int32_t num_kv_heads,
+                                int32_t head_dim, int32_t block_size, int32_t max_blocks_per_seq, int32_t dtype);
+int mip_paged_tree(void* out, int64_t out_stride_tok, int64_t out_stride_head, const void* q, int64_t q_stride_tok,
+                   int64_t q_stride_head, const void* k_cache, const void* v_cache, int64_t num_cache_blocks,
+                   const int32_t* block_tables, int64_t bt_stride, const int32_t* cu_q, const int32_t* ctx_start,
+                   const uint64_t* mask, int64_t mask_stride, int32_t mask_words, int32_t num_seqs, int32_t max_q_len,
+                   int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                   int32_t max_blocks_per_seq, float scale, void* workspace, size_t workspace_bytes, int32_t dtype,
+                   void* stream);
+
+/*
+ * mip_tree_index: from the trees' parents (parents[r]: the parent's number in its tree, below i; any other
+ * value makes the node a root),
+ *     positions[r]    = c + depth of node i (a root has depth 0)
+ *     slot_mapping[r] = pool slot of cache index c + i, -1 past the table
+ *     mask[r]         = the nodes on the path from i to its root, i among them, mask_words words a row
+ * max_q_len at most MIP_TREE_MAX_NODES (MIP_EUNSUPPORTED).
+ */
+#define MIP_TREE_MAX_NODES 1024
+int mip_tree_index(int64_t* positions, int64_t* slot_mapping, uint64_t* mask, int32_t mask_words,
+                   const int32_t* parents, const int32_t* cu_q, const int32_t* ctx_start, const int32_t* block_tables,
+                   int64_t bt_stride, int32_t num_seqs, int32_t max_q_len, int32_t block_size,
+                   int32_t max_blocks_per_seq, void* stream);
+
+/*
+ * mip_tree_verify: greedy verification against the logits [n_rows][vocab] (row_stride elements).
+ *     target[r]     = the lowest index of row r's greatest logit (NaN counts as the greatest), all n_rows rows
+ *     path[s]       = node 0, then from each node on to its lowest child (parents[r] = that node) whose
+ *                     token tokens[r] is the node's target, until there is none; -1 from counts[s] on
+ *     next_token[s] = target of the path's last node (-1, with counts[s] = 0, for an empty tree)
+ * path has max_q_len entries a sequence; max_q_len at most MIP_TREE_MAX_NODES. The workspace holds
+ * mip_tree_verify_workspace(..) bytes, 8-byte aligned.
+ */
+size_t mip_tree_verify_workspace(int32_t n_rows, int32_t vocab, int32_t dtype);
+int mip_tree_verify(int64_t* target, int32_t* path, int32_t* counts, int64_t* next_token, const void* logits,
+                    int64_t row_stride, int32_t n_rows, int32_t vocab, const int64_t* tokens, const int32_t* parents,
+                    const int32_t* cu_q, int32_t num_seqs, int32_t max_q_len, void* workspace, size_t workspace_bytes,
+                    int32_t dtype, void* stream);
+
+/*
+ * mip_tree_commit: for d < counts[s], every layer, K and V, the row of cache index c + path[s][d] is
+ * moved to cache index c + d, bit for bit, as if all rows were read before any is written. Paths rise
+ * and have path[s][d] >= d (as mip_tree_verify's do); an entry that does not, or whose place lies outside the
+ * table or the pool, ends its path. The pools are whole ([num_layers] layers of num_cache_blocks blocks);
+ * no two sequences may share a block from cache index c on.
+ */
+int mip_tree_commit(void* k_pool, void* v_pool, int32_t num_layers, int64_t num_cache_blocks, int32_t num_kv_heads,
+                    int32_t head_dim, int32_t block_size, const int32_t* block_tables, int64_t bt_stride,
+                    int32_t max_blocks_per_seq, const int32_t* ctx_start, const int32_t* path, int64_t path_stride,
+                    int32_t max_path, const int32_t* counts, int32_t num_seqs, int32_t dtype, void* stream);
 
 /*
  * The layer calls of one step. Every layer of a step passes the same sequences, strides and sizes

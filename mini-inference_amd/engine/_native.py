@@ -15,6 +15,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libmipaged.so"
 MIP_F32, MIP_F16, MIP_BF16 = 0, 1, 2
 MIP_OK, MIP_E2BIG, MIP_EINVAL, MIP_EUNSUPPORTED = 0, -7, -22, -95
 MIP_NOALLOC_SCRATCH_BYTES = 32 << 20
+MIP_TREE_MAX_NODES = 1024
 MIP_ALGO = {"auto": 0, "valu": 1, "mfma": 2, "stream": 3}
 
 EXPORTED = (
@@ -45,6 +46,12 @@ EXPORTED = (
     "mip_norm_linear",
     "mip_qkv_linear",
     "mip_linear_residual",
+    "mip_paged_tree",
+    "mip_paged_tree_workspace",
+    "mip_tree_index",
+    "mip_tree_verify",
+    "mip_tree_verify_workspace",
+    "mip_tree_commit",
 )
 
 # Measurement helpers in the same library (include/mipaged_probe.h), outside the drop-in ABI.
@@ -141,6 +148,22 @@ _SIGNATURES = {
     "mip_norm_linear": (_c.c_int, [_vp, _vp, _vp, _f32, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp]),
     "mip_qkv_linear": (_c.c_int, [_vp, _vp, _vp, _f32, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _vp]),
     "mip_linear_residual": (_c.c_int, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp]),
+    "mip_paged_tree": (
+        _c.c_int,
+        [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64,
+         _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _vp, _sz, _i32, _vp],
+    ),
+    "mip_paged_tree_workspace": (_sz, [_i32] * 8),
+    "mip_tree_index": (_c.c_int, [_vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp]),
+    "mip_tree_verify": (
+        _c.c_int,
+        [_vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _i32, _i32, _vp, _sz, _i32, _vp],
+    ),
+    "mip_tree_verify_workspace": (_sz, [_i32, _i32, _i32]),
+    "mip_tree_commit": (
+        _c.c_int,
+        [_vp, _vp, _i32, _i64, _i32, _i32, _i32, _vp, _i64, _i32, _vp, _vp, _i64, _i32, _vp, _i32, _i32, _vp],
+    ),
     "mip_hbm_read_probe": (_c.c_int, [_vp, _i64, _vp, _i64, _i32, _vp, _i32, _i32, _vp]),
 }
 

@@ -729,3 +729,225 @@ def copy_blocks(k_pool: torch.Tensor, v_pool: torch.Tensor, pairs) -> None:
     Bitwise copy (no reference counterpart; used for copy-on-write of shared prefix blocks).
     """
     prepare_copy_blocks(k_pool, v_pool, pairs)()
+
+
+def _one_device(*tensors: torch.Tensor) -> torch.device:
+    """The device that all of these are on; a call whose pointers belong to several is refused."""
+    device = tensors[0].device
+    for t in tensors:
+        if t.device != device:
+            raise ValueError(f"tensors on different devices: {device} and {t.device}")
+    _require_device(tensors[0])
+    return device
+
+
+def _call_on(device: torch.device, fn, args: tuple, what: str) -> None:
+    """Launch on the current stream of ``device``, whichever device is current."""
+    if device.index == torch.cuda.current_device():
+        st = fn(*args, _stream_ptr(device))
+    else:
+        with torch.cuda.device(device):
+            st = fn(*args, _stream_ptr(device))
+    if st:
+        _native.check(st, what)
+
+
+def _tree_rows(cu_q: torch.Tensor, block_tables: torch.Tensor, ctx_start: torch.Tensor, max_q_len: int,
+               max_blocks: int | None) -> tuple[int, int]:
+    """Check the tensors that describe a step of trees; returns (sequences, blocks of a table)."""
+    if not cu_q.dtype == ctx_start.dtype == block_tables.dtype == torch.int32:
+        raise TypeError("cu_q, ctx_start and block_tables must be int32")
+    if ctx_start.dim() != 1 or cu_q.shape != (ctx_start.shape[0] + 1,):
+        raise ValueError("cu_q must be int32 [S + 1] and ctx_start int32 [S]")
+    s = ctx_start.shape[0]
+    if block_tables.dim() != 2 or block_tables.shape[0] < s or block_tables.shape[1] < 1:
+        raise ValueError("block_tables must be int32 [S, max_blocks]")
+    if not (cu_q.is_contiguous() and ctx_start.is_contiguous()) or block_tables.stride(1) != 1:
+        raise ValueError("cu_q, ctx_start and the block_tables rows must be contiguous")
+    if max_q_len < 0:
+        raise ValueError(f"max_q_len={max_q_len} is negative")
+    mb = block_tables.shape[1] if max_blocks is None else int(max_blocks)
+    if mb < 1 or mb > block_tables.shape[1]:
+        raise ValueError(f"max_blocks={mb} is outside [1, {block_tables.shape[1]}]")
+    return s, mb
+
+
+def _scratch(workspace: torch.Tensor | None, device: torch.device, need: int) -> tuple[int | None, int]:
+    """Address and size of a call's scratch memory: the caller's, or the device's shared buffer."""
+    if workspace is None:
+        workspace = _workspace.get(device, need)
+    elif need and workspace.numel() * workspace.element_size() < need:
+        raise ValueError(f"workspace holds {workspace.numel() * workspace.element_size()} bytes, needs {need}")
+    elif workspace.device != device or not workspace.is_contiguous():
+        raise ValueError("workspace must be a contiguous tensor on the call's device")
+    if workspace is None:
+        return None, 0
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+def tree_index(parents: torch.Tensor, cu_q: torch.Tensor, ctx_start: torch.Tensor, block_tables: torch.Tensor,
+               max_q_len: int, block_size: int,
+               max_blocks: int | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Where the nodes of drafted trees go and what they see: ``(positions, slot_mapping, mask)``.
+
+    Node i of sequence s is packed row ``cu_q[s] + i`` (int32 ``[S + 1]``); ``parents`` (int32 ``[N]``) holds
+    each node's parent by its number in the tree, which is below the node's own (anything else: a
+    root). ``positions`` (int64 ``[N]``) are ``ctx_start[s]`` + depth; ``slot_mapping`` (int64 ``[N]``) the
+    pool slots of cache indexes ``ctx_start[s] + i`` (-1 past the table); ``mask`` (int64 ``[N, W]``,
+    ``W = ceil(max_q_len / 64)``) has bit ``j % 64`` of word ``j // 64`` set for the nodes j on the path to the
+    root, the node itself among them: what :func:`paged_tree` takes. Trees of up to 1024 nodes. Rows of
+    no sequence are not written.
+    """
+    s, mb = _tree_rows(cu_q, block_tables, ctx_start, max_q_len, max_blocks)
+    if parents.dtype != torch.int32 or parents.dim() != 1 or not parents.is_contiguous():
+        raise ValueError("parents must be contiguous int32 [N]")
+    device = _one_device(parents, cu_q, ctx_start, block_tables)
+    n, words = parents.shape[0], (max_q_len + 63) // 64
+    both = torch.empty(2 * n, dtype=torch.int64, device=device)
+    mask = torch.empty(n, words, dtype=torch.int64, device=device)
+    positions, slots = both[:n], both[n:]
+    if n and s and max_q_len:
+        _call_on(device, _native.load().mip_tree_index,
+                 (positions.data_ptr(), slots.data_ptr(), mask.data_ptr(), words, parents.data_ptr(), cu_q.data_ptr(),
+                  ctx_start.data_ptr(), block_tables.data_ptr(), block_tables.stride(0), s, max_q_len, block_size, mb),
+                 "mip_tree_index")
+    return positions, slots, mask
+
+
+def paged_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+               cu_q: torch.Tensor, ctx_start: torch.Tensor, mask: torch.Tensor, max_q_len: int,
+               scale: float | None = None, out: torch.Tensor | None = None, max_blocks: int | None = None,
+               workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of drafted trees' nodes over their sequences' paged keys and each other.
+
+    ``q``: ``[N, Hq, D]`` packed rows (last dim contiguous); sequence ``s`` owns rows ``cu_q[s] ..
+    cu_q[s + 1] - 1`` (int32 ``[S + 1]``), whose keys and values are in the pool at cache indexes
+    ``ctx_start[s] + i`` (int32 ``[S]``; append them first). A row sees its sequence's ``ctx_start[s]`` cached keys and
+    the nodes that its bits in ``mask`` (int64 ``[N, W]``, ``W >= ceil(max_q_len / 64)``, rows contiguous) name; a row that sees
+    nothing becomes zeros, and what a row does not see has no influence on it. Returns ``out [N, Hq, D]``; rows of no
+    sequence are not written. No reference counterpart (one token a step there, engine/kv_cache.py:615-620).
+
+    16-bit types at head_dim 64 / 128 run on the matrix cores, long contexts of few rows cut into pieces and
+    combined; other types and head sizes (powers of two from 8 to 256) one query row at a time. Scratch
+    memory is shared by the calls of a device, which must then be ordered; pass ``workspace``
+    (:func:`tree_workspace_bytes`) to calls that may run at once.
+    """
+    if q.dim() != 3 or q.stride(2) != 1:
+        raise ValueError("q must be [N, Hq, D] with a contiguous last dimension")
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError("k_cache/v_cache must be contiguous [num_blocks, Hkv, block_size, D] tensors of one shape")
+    nb, hkv, bs, d = k_cache.shape
+    n, hq, dq = q.shape
+    if dq != d or hkv == 0 or hq == 0 or hq % hkv:
+        raise ValueError(f"q {tuple(q.shape)} does not match the pool (Hkv={hkv}, D={d})")
+    if q.dtype != k_cache.dtype or v_cache.dtype != k_cache.dtype:
+        raise TypeError("q and the cache must share one dtype")
+    s, mb = _tree_rows(cu_q, block_tables, ctx_start, max_q_len, max_blocks)
+    words = (max_q_len + 63) // 64
+    if mask.dtype != torch.int64 or mask.dim() != 2 or mask.shape[0] != n or mask.shape[1] < words or (
+            mask.shape[1] > 1 and mask.stride(1) != 1):
+        raise ValueError(f"mask must be int64 [{n}, >= {words}] with contiguous rows, got {tuple(mask.shape)} {mask.dtype}")
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    if not scale > 0.0:
+        raise ValueError(f"scale={scale} must be positive")
+    if out is None:
+        out = torch.empty((n, hq, d), dtype=q.dtype, device=q.device)
+    elif out.shape != (n, hq, d) or out.dtype != q.dtype or out.stride(2) != 1:
+        raise ValueError("out must be [N, Hq, D] in q's dtype with a contiguous last dimension")
+    device = _one_device(q, k_cache, v_cache, block_tables, cu_q, ctx_start, mask, out)
+    if not (n and s and max_q_len):
+        return out
+    code, lib = dtype_code(q.dtype), _native.load()
+    ws_ptr, ws_bytes = _scratch(workspace, device, int(lib.mip_paged_tree_workspace(s, max_q_len, hq, hkv, d, bs, mb, code)))
+    _call_on(device, lib.mip_paged_tree,
+             (out.data_ptr(), out.stride(0), out.stride(1), q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
+              v_cache.data_ptr(), nb, block_tables.data_ptr(), block_tables.stride(0), cu_q.data_ptr(),
+              ctx_start.data_ptr(), mask.data_ptr(), mask.stride(0), mask.shape[1], s, max_q_len, hq, hkv, d, bs, mb,
+              scale, ws_ptr, ws_bytes, code), "mip_paged_tree")
+    return out
+
+
+def tree_workspace_bytes(num_seqs: int, max_q_len: int, num_heads: int, num_kv_heads: int, head_dim: int,
+                         block_size: int, max_blocks: int, dtype: torch.dtype) -> int:
+    """Bytes of scratch a :func:`paged_tree` call of this shape needs (``mip_paged_tree_workspace``)."""
+    return int(_native.load().mip_paged_tree_workspace(num_seqs, max_q_len, num_heads, num_kv_heads, head_dim,
+                                                       block_size, max_blocks, dtype_code(dtype)))
+
+
+def tree_verify(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, cu_q: torch.Tensor, max_q_len: int,
+                workspace: torch.Tensor | None = None
+                ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Greedy verification of drafted trees: ``(target, path, counts, next_token)``.
+
+    ``logits`` ``[N, vocab]`` (rows contiguous): the model's answer after every node; ``tokens`` int64 ``[N]`` the
+    nodes' tokens, ``parents`` and ``cu_q`` as for :func:`tree_index`. ``target`` (int64 ``[N]``): the lowest index
+    of each row's greatest logit (a NaN counts as the greatest). ``path`` (int32 ``[S, max_q_len]``, -1 past the
+    end) starts at node 0 and goes on to the lowest child whose token is the last node's target, until there is none;
+    ``counts`` (int32 ``[S]``) are the paths' lengths and ``next_token`` (int64 ``[S]``) the target of each one's last node
+    (an empty tree: 0 and -1). Scratch memory as for :func:`paged_tree`.
+    """
+    if logits.dim() != 2 or logits.shape[1] < 1 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("logits must be [N, vocab] with contiguous rows")
+    n, vocab = logits.shape
+    code = dtype_code(logits.dtype)
+    if tokens.dtype != torch.int64 or tokens.shape != (n,) or not tokens.is_contiguous():
+        raise ValueError(f"tokens must be contiguous int64 [{n}]")
+    if parents.dtype != torch.int32 or parents.shape != (n,) or not parents.is_contiguous():
+        raise ValueError(f"parents must be contiguous int32 [{n}]")
+    if cu_q.dtype != torch.int32 or cu_q.dim() != 1 or cu_q.shape[0] < 1 or not cu_q.is_contiguous():
+        raise ValueError("cu_q must be contiguous int32 [S + 1]")
+    if max_q_len < 0:
+        raise ValueError(f"max_q_len={max_q_len} is negative")
+    device = _one_device(logits, tokens, parents, cu_q)
+    s, row_stride = cu_q.shape[0] - 1, max(logits.stride(0), vocab) if n <= 1 else logits.stride(0)
+    if row_stride < vocab:
+        raise ValueError("the rows of logits overlap")
+    both = torch.empty(n + s, dtype=torch.int64, device=device)
+    ints = torch.empty(s * max_q_len + s, dtype=torch.int32, device=device)
+    target, following = both[:n], both[n:]
+    path, counts = ints[:s * max_q_len].view(s, max_q_len), ints[s * max_q_len:]
+    if n or s:
+        lib = _native.load()
+        ws_ptr, ws_bytes = _scratch(workspace, device, int(lib.mip_tree_verify_workspace(n, vocab, code)))
+        _call_on(device, lib.mip_tree_verify,
+                 (target.data_ptr(), path.data_ptr(), counts.data_ptr(), following.data_ptr(), logits.data_ptr(),
+                  row_stride, n, vocab, tokens.data_ptr(), parents.data_ptr(), cu_q.data_ptr(), s, max_q_len, ws_ptr,
+                  ws_bytes, code), "mip_tree_verify")
+    return target, path, counts, following
+
+
+def tree_commit(k_pool: torch.Tensor, v_pool: torch.Tensor, block_tables: torch.Tensor, ctx_start: torch.Tensor,
+                path: torch.Tensor, counts: torch.Tensor, max_blocks: int | None = None) -> None:
+    """Move the accepted nodes' keys and values to the places of consecutive tokens, every layer, in place.
+
+    ``k_pool``/``v_pool``: ``[num_layers, num_blocks + 1, Hkv, block_size, D]`` contiguous. ``path`` (int32 ``[S, P]``) and
+    ``counts`` (int32 ``[S]``) as :func:`tree_verify` returns them: the row of cache index ``ctx_start[s] + path[s, d]``
+    moves to ``ctx_start[s] + d`` for ``d < counts[s]``, as if all were read before any is written. A path rises and
+    has ``path[s, d] >= d``; an entry that breaks this, or whose place lies outside the table or the pool, ends it.
+    """
+    if k_pool.dim() != 5 or k_pool.shape != v_pool.shape or not (k_pool.is_contiguous() and v_pool.is_contiguous()):
+        raise ValueError("k_pool/v_pool must be contiguous [L, num_blocks, Hkv, block_size, D] tensors of one shape")
+    if k_pool.dtype != v_pool.dtype:
+        raise TypeError("the pools must share one dtype")
+    if not path.dtype == counts.dtype == ctx_start.dtype == block_tables.dtype == torch.int32:
+        raise TypeError("path, counts, ctx_start and block_tables must be int32")
+    s = counts.numel()
+    if counts.dim() != 1 or ctx_start.shape != (s,) or path.dim() != 2 or path.shape[0] != s:
+        raise ValueError("path must be int32 [S, P], counts and ctx_start int32 [S]")
+    if block_tables.dim() != 2 or block_tables.shape[0] < s or block_tables.shape[1] < 1 or block_tables.stride(1) != 1:
+        raise ValueError("block_tables must be int32 [S, max_blocks] with contiguous rows")
+    if not (counts.is_contiguous() and ctx_start.is_contiguous()) or (path.shape[1] > 1 and path.stride(1) != 1) or (
+            s > 1 and path.stride(0) < path.shape[1]):
+        raise ValueError("counts, ctx_start and the rows of path must be contiguous")
+    mb = block_tables.shape[1] if max_blocks is None else int(max_blocks)
+    if mb < 1 or mb > block_tables.shape[1]:
+        raise ValueError(f"max_blocks={mb} is outside [1, {block_tables.shape[1]}]")
+    layers, nb, hkv, bs, d = k_pool.shape
+    code = dtype_code(k_pool.dtype)
+    device = _one_device(k_pool, v_pool, block_tables, ctx_start, path, counts)
+    if s == 0 or path.shape[1] == 0:
+        return
+    _call_on(device, _native.load().mip_tree_commit,
+             (k_pool.data_ptr(), v_pool.data_ptr(), layers, nb, hkv, d, bs, block_tables.data_ptr(),
+              block_tables.stride(0), mb, ctx_start.data_ptr(), path.data_ptr(), max(path.stride(0), path.shape[1]),
+              path.shape[1], counts.data_ptr(), s, code), "mip_tree_commit")
