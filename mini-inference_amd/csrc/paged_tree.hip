@@ -46,6 +46,10 @@ using decode::fast_exp2;
 using decode::kRescaleLog2;
 using decode::MfmaOps;
 
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint4 u4(const u32x4_t& x) { return __builtin_bit_cast(uint4, x); }
+
 constexpr int kMaxSeqs = 1024;  // sequences whose places fit in LDS
 
 struct TreeArgs {
@@ -66,15 +70,10 @@ struct TreeArgs {
   int hkv, group, bs, log2_bs, max_blocks;
   int num_seqs, max_q_len;
   float scale_log2;
-  // Split segments: record g (m[R] | l[R] | acc) at ws_rec + g * rec_floats, its segment's descriptor
-  // at ws_desc + g * kDesc, written by the segment's first piece and invalid (pieces 0) elsewhere.
-  float* ws_rec;
-  int32_t* ws_desc;
-  int64_t rec_floats;
-  int target, min_steps, max_recs;
+  int min_share;           // fewest steps a worker takes
+  float* ws_rec;           // two records a worker: m[R] | l[R] | accumulators
+  int32_t* ws_start;       // first step of every sequence, then the steps of a share (null: no segment is split)
 };
-
-constexpr int kDesc = 4;  // words: pieces, sequence, kv head, row block
 
 __device__ __forceinline__ float fmax2(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 __device__ __forceinline__ float fmax3(float a, float b, float c) { return fmax2(fmax2(a, b), c); }
@@ -95,26 +94,13 @@ __device__ __forceinline__ uint2 lds_tr16(const char* p) {
 
 // Eight bf16 values -> fp16: exact from 2^-17 to 65280 in magnitude, inf from 65536 on; smaller ones land
 // on fp16's subnormal grid (a change of at most 2^-25).
-__device__ __forceinline__ uint4 bf16x8_to_f16x8(const uint4& v) {
+__device__ __forceinline__ u32x4_t bf16x8_to_f16x8(const u32x4_t& v) {
   auto cv = [](uint32_t x) __attribute__((always_inline)) {
     return MfmaOps<MIP_F16>::pack2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
   };
-  return make_uint4(cv(v.x), cv(v.y), cv(v.z), cv(v.w));
+  return u32x4_t{cv(v[0]), cv(v[1]), cv(v[2]), cv(v[3])};
 }
 
-// A pair of 16-bit values with inf and NaN replaced by 0; `wild` is set if there was one.
-template <int DT> __device__ __forceinline__ uint32_t finite2(uint32_t x, bool& wild) {
-  constexpr uint32_t kExp = DT == MIP_BF16 ? 0x7f80u : 0x7c00u;
-  if ((x & kExp) == kExp) {
-    x &= 0xffff0000u;
-    wild = true;
-  }
-  if (((x >> 16) & kExp) == kExp) {
-    x &= 0xffffu;
-    wild = true;
-  }
-  return x;
-}
 
 template <int D, int WR, int WK, int NC>
 struct Shape {
@@ -126,82 +112,448 @@ struct Shape {
   static constexpr int CPR = RB / 16;              // 16-byte chunks of a row
   static constexpr int KC = D / 32, MT = D / 16;
   static constexpr int TILE = KT * RB;             // bytes of a step's K (or V)
-  static constexpr int STAGE = 2 * TILE;
-  static constexpr int NLD = KT * CPR / T;         // chunks a thread copies, each of K and V
+  static constexpr bool kPrivate = WR == 1;        // wavefronts share no keys: each fetches its own
+  static constexpr int STAGE = 2 * TILE;           // shared: K | V of a step
+  static constexpr int NLD = KT * CPR / T;         // shared: chunks a thread copies, each of K and V
+  static constexpr int kRing = 2 * 64 * RB;        // private: a wavefront's two tiles of 32 K and 32 V rows
+  // The meeting of the WK wavefronts of a row goes through LDS one column block at a time.
+  static constexpr int kPark = NW * MT * kWave * 16;
+  static constexpr int kStages = kPrivate ? NW * kRing : 2 * STAGE;
+  static constexpr int kLds = WK > 1 && kPark > kStages ? kPark : kStages;
   static constexpr int64_t kRec = 2 * R + static_cast<int64_t>(R) * D;  // floats of a record
-  static_assert(NLD >= 1 && NLD * T == KT * CPR, "a step splits evenly over the threads");
-  // The meeting of the WK wavefronts of a row reuses the stages.
-  static_assert(WK == 1 || WR * (WK - 1) * NC * MT * kWave * 16 <= 2 * STAGE, "accumulators must fit");
-  // V row r keeps chunk c at c ^ vsw(r): even, so that each 32-byte segment of a transposing read stays
-  // whole, and the 8 rows that 32 lanes read start in distinct banks.
-  static __device__ __forceinline__ int vsw(int r) { return CPR >= 16 ? 2 * (r & 7) : 2 * ((r + (r >> 2)) & 3); }
+  static_assert(NW == 4 && KT * CPR % T == 0 && MT % WK == 0, "a step splits evenly over four wavefronts");
+};
+
+// V row r keeps chunk c at c ^ vsw(r): even, so that each 32-byte segment of a transposing read stays whole,
+// and the 8 rows that 32 lanes read start in distinct banks.
+template <int D> __device__ __forceinline__ int vsw(int r) { return D >= 128 ? 2 * (r & 7) : 2 * ((r + (r >> 2)) & 3); }
+
+struct Seq {
+  int q0, n, ctx;
 };
 
 struct Piece {
-  int s, kvh, rb, q0, n, ctx, keys, step0, step1;
+  Seq q;
+  int s, kvh, rb, last, step0, step1;  // last: the last key's index
 };
 
 // What a workgroup shares beside the stages.
-template <int T, int NW, int ML>
 struct Shared {
-  int scan[2][NW];
-  int pieces[kMaxSeqs + 1], recs[kMaxSeqs + 1];  // exclusive prefixes over the sequences
-  uint32_t ok[2];      // byte w: every key that wavefront w copied lies in a block of the pool
-  uint32_t wild[2];    // careful pass: byte w: wavefront w copied an inf or NaN value
-  uint32_t tag;        // of the piece that has to run again
-  float ml[2][ML];     // maxima and sums of the WK - 1 other wavefronts of each row
+  int scan[4];
+  int start[kMaxSeqs];  // first step of every sequence's segments
+  uint32_t ok[2];       // byte w: every key that wavefront w copied exists and lies in a block of the pool
 };
 
-__device__ __forceinline__ Piece seq_shape(const TreeArgs& a, int s, int cap) {
-  Piece p;
-  p.s = s;
-  p.q0 = a.cu_q[s];
-  p.n = a.cu_q[s + 1] - p.q0;
-  p.n = p.n < a.max_q_len ? p.n : a.max_q_len;
-  p.n = p.n > 0 ? p.n : 0;
-  p.ctx = a.ctx_start[s];
-  p.ctx = p.ctx > 0 ? p.ctx : 0;
-  p.keys = p.ctx < cap - p.n ? p.ctx + p.n : cap;  // keys past the table are never read
-  return p;
+__device__ __forceinline__ Seq seq_of(const TreeArgs& a, int s) {
+  Seq q;
+  q.q0 = a.cu_q[s];
+  q.n = a.cu_q[s + 1] - q.q0;
+  q.n = q.n < a.max_q_len ? q.n : a.max_q_len;
+  q.n = q.n > 0 ? q.n : 0;
+  q.ctx = a.ctx_start[s];
+  q.ctx = q.ctx > 0 ? q.ctx : 0;
+  return q;
 }
 
-// One piece: rows of block p.rb against steps [p.step0, p.step1). Returns true (and writes nothing) if it has
-// to run again with CAREFUL. rec < 0: the piece is its whole segment and writes the output.
-template <int DT, int D, int WR, int WK, int NC, bool CAREFUL, class Sh>
-__device__ __forceinline__ bool run_piece(const TreeArgs& a, const Piece& p, int64_t rec, uint32_t tag, char* smem,
-                                          Sh& sh) {
-  using P = Shape<D, WR, WK, NC>;
-  constexpr bool VF16 = DT == MIP_BF16 && !CAREFUL;
-  using Ops = MfmaOps<DT>;
-  using OpsV = MfmaOps<VF16 ? MIP_F16 : DT>;
-  constexpr int RB = P::RB, CPR = P::CPR, KC = P::KC, MT = P::MT, NLD = P::NLD;
-  const int tid = threadIdx.x, lane = tid & (kWave - 1);
-  const int w = __builtin_amdgcn_readfirstlane(tid / kWave);
-  const int wr = w / WK, wk = w - wr * WK;
-  const int i16 = lane & 15, grp = lane >> 4;
-  const int G = a.group, last = p.keys - 1;
-  const int32_t* table = a.bt + static_cast<int64_t>(p.s) * a.bt_stride;
+// Keys of a sequence; those past the table are never read.
+__device__ __forceinline__ int keys_of(const TreeArgs& a, const Seq& q) {
+  const int cap = a.max_blocks * a.bs;
+  return q.ctx < cap - q.n ? q.ctx + q.n : cap;
+}
 
-  // ---- this lane's query row in each column block.
+// The query rows of a wavefront: row 16 c + lane % 16 of its NC column blocks, with its running softmax.
+template <int D, int NC>
+struct Rows {
+  static constexpr int KC = D / 32, MT = D / 16;
+  u32x4_t q[NC][KC];  // Q^T operand; zeros in rows that are none
+  int tok[NC];        // node (0 in rows that are none)
   bool live[NC];
-  int tok[NC];
-  uint4 qreg[NC][KC];
+  f32x4_t acc[NC][MT];
+  f32x4_t l[NC];      // row sums by MFMA against a block of ones: every element holds the row's
+  float m[NC];        // running maximum (log2 units)
+
+  __device__ __forceinline__ void load(const TreeArgs& a, const Piece& p, int first, int i16, int grp) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int r = first + c * 16 + i16;
+      const int t = r / a.group, g = r - t * a.group;
+      live[c] = t < p.q.n;
+      tok[c] = live[c] ? t : 0;
+      const char* row = a.q + ((static_cast<int64_t>(p.q.q0) + tok[c]) * a.q_st +
+                               static_cast<int64_t>(p.kvh * a.group + (live[c] ? g : 0)) * a.q_sh) * 2;
+#pragma unroll
+      for (int kc = 0; kc < KC; ++kc)
+        q[c][kc] = live[c] ? *reinterpret_cast<const u32x4_t*>(row + (32 * kc + 8 * grp) * 2) : u32x4_t{0, 0, 0, 0};
+    }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      m[c] = -INFINITY;
+      l[c] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) acc[c][mt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+  }
+  __device__ __forceinline__ bool finite() const {  // of the whole wavefront
+    float big = 0.0f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+        big = fmax3(big, fmax2(fabsf(acc[c][mt][0]), fabsf(acc[c][mt][1])),
+                    fmax2(fabsf(acc[c][mt][2]), fabsf(acc[c][mt][3])));
+    // On the bits: the compiler takes a maximum of absolute values for a number and compares it as one.
+    return __all(__float_as_uint(big) < 0x7f800000u);
+  }
+};
+
+// The nodes among keys key0 .. key0 + 31 that a mask row names, as bits; cached keys (below ctx) are all set.
+__device__ __forceinline__ uint32_t mask_window(const TreeArgs& a, const Piece& p, int tok, int key0) {
+  const int e0 = key0 - p.q.ctx;  // tree number of the first key (below 0: cached)
+  if (e0 <= -32) return 0xffffffffu;
+  const uint64_t* row = a.mask + (static_cast<int64_t>(p.q.q0) + tok) * a.mask_st;
+  if (e0 < 0) return static_cast<uint32_t>(row[0] << -e0) | ((1u << -e0) - 1u);
+  const int word = e0 >> 6, off = e0 & 63;
+  uint64_t x = word < a.mask_words ? row[word] >> off : 0;
+  if (off > 32 && word + 1 < a.mask_words) x |= row[word + 1] << (64 - off);
+  return static_cast<uint32_t>(x);
+}
+
+// Scores of 32 keys against a wavefront's rows, masked, and the rows' maxima brought up to date. k: the K operand of
+// the two 16-key halves (lane: key 16 u + lane % 16, dims 32 kc + 8 (lane / 16) ..). real: bit k: key key0 + k
+// exists and lies in the pool. sv[c][i]: row lane % 16 of block c against key 4 (lane / 16) + kKey[i].
+constexpr int kKey[8] = {0, 1, 2, 3, 16, 17, 18, 19};
+template <int DT, int D, int NC>
+__device__ __forceinline__ void score_tile(const TreeArgs& a, const Piece& p, Rows<D, NC>& rows, const u32x4_t (&k)[2][D / 32],
+                                           int key0, uint32_t real, int grp, float (&sv)[NC][8]) {
+  constexpr int KC = D / 32, MT = D / 16;
+  using Ops = MfmaOps<DT>;
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    const int r = p.rb * P::R + (wr * NC + c) * 16 + i16;
-    const int t = r / G, g = r - t * G;
-    live[c] = t < p.n;
-    tok[c] = live[c] ? t : 0;
-    const char* qrow = a.q + ((static_cast<int64_t>(p.q0) + tok[c]) * a.q_st +
-                              static_cast<int64_t>(p.kvh * G + (live[c] ? g : 0)) * a.q_sh) * 2;
+    f32x4_t s0 = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}, s1 = s0;
 #pragma unroll
-    for (int kc = 0; kc < KC; ++kc)
-      qreg[c][kc] = live[c] ? *reinterpret_cast<const uint4*>(qrow + (32 * kc + 8 * grp) * 2) : make_uint4(0, 0, 0, 0);
+    for (int kc = 0; kc < KC; ++kc) {
+      s0 = Ops::qk(u4(k[0][kc]), u4(rows.q[c][kc]), s0);
+      s1 = Ops::qk(u4(k[1][kc]), u4(rows.q[c][kc]), s1);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sv[c][i] = i < 4 ? s0[i] : s1[i - 4];
   }
+  if (real != 0xffffffffu || key0 + 31 >= p.q.ctx) {  // else: cached keys only, which everybody sees
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const uint32_t mine = (rows.live[c] ? mask_window(a, p, rows.tok[c], key0) & real : 0u) >> (4 * grp);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sv[c][i] = (mine >> kKey[i]) & 1u ? sv[c][i] : -INFINITY;
+    }
+  }
+  // One wave-uniform test decides whether any row's maximum rises by more than kRescaleLog2; most tiles raise none.
+  float mx[NC];
+  bool need = false;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    mx[c] = fmax3(fmax3(sv[c][0], sv[c][1], sv[c][2]), fmax3(sv[c][3], sv[c][4], sv[c][5]), fmax2(sv[c][6], sv[c][7])) *
+            a.scale_log2;
+    need = need || mx[c] > rows.m[c] + kRescaleLog2;
+  }
+  if (__any(need)) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      if (__any(mx[c] > rows.m[c] + kRescaleLog2)) {
+        const float mn = fmax2(rows.m[c], max4(mx[c]));
+        const float alpha = rows.m[c] == -INFINITY ? 0.0f : fast_exp2(rows.m[c] - mn);
+        rows.l[c] *= alpha;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) rows.acc[c][mt] *= alpha;
+        rows.m[c] = mn;
+      }
+    }
+  }
+}
 
-  // ---- loader: block ids one step ahead of the rows, rows one step ahead of their use.
-  uint4 kbuf[NLD], vbuf[NLD];
-  bool okbuf[NLD];
+// The weights of block c from its scores: exp2(-inf - m) = 0 for a finite m; m stays -inf only while every score of the
+// row is -inf, and then 0 stands for it.
+__device__ __forceinline__ void weights(const float (&sv)[8], float m, float scale_log2, float (&pr)[8]) {
+  const float nm = m == -INFINITY ? 0.0f : -m;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) pr[i] = fast_exp2(fmaf(sv[i], scale_log2, nm));
+}
+
+template <class Ops> __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
+  return make_uint4(Ops::pack2(x[0], x[1]), Ops::pack2(x[2], x[3]), Ops::pack2(x[4], x[5]), Ops::pack2(x[6], x[7]));
+}
+
+// The weights' products with V^T and their sums. vt: lane (dim 16 mt + lane % 16): k index 8 grp + i stands for key
+// 4 grp + i (i < 4) or 16 + 4 grp + i - 4, the keys of this lane's scores, so the weights stay where they are. VT: the
+// type of V in vt. Weights enter as VT, for bf16 with their rounding remainders as a second product.
+template <int VT, int D, int NC>
+__device__ __forceinline__ void value_tile(Rows<D, NC>& rows, const u32x4_t (&vt)[D / 16], const float (&sv)[NC][8],
+                                           float scale_log2) {
+  constexpr int MT = D / 16;
+  using Ops = MfmaOps<VT>;
+  constexpr uint32_t kOne2 = VT == MIP_BF16 ? 0x3f803f80u : 0x3c003c00u;
+  const uint4 ones = make_uint4(kOne2, kOne2, kOne2, kOne2);
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    float pr[8];
+    weights(sv[c], rows.m[c], scale_log2, pr);
+    const uint4 ph = pack8<Ops>(pr);
+    rows.l[c] = Ops::qk(ones, ph, rows.l[c]);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) rows.acc[c][mt] = Ops::qk(u4(vt[mt]), ph, rows.acc[c][mt]);
+    if constexpr (VT == MIP_BF16) {
+      const uint32_t h[4] = {ph.x, ph.y, ph.z, ph.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) pr[i] -= i & 1 ? Ops::hi(h[i / 2]) : Ops::lo(h[i / 2]);
+      const uint4 pl = pack8<Ops>(pr);
+      rows.l[c] = Ops::qk(ones, pl, rows.l[c]);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) rows.acc[c][mt] = Ops::qk(u4(vt[mt]), pl, rows.acc[c][mt]);
+    }
+  }
+}
+
+// A wavefront's keys of a piece (32 at wk * 32 of every step of KT), for sums that ended as inf or NaN: the same
+// softmax, each value added to the rows that see its key alone (0 * inf of a masked key must not reach a row), in fp32
+// with the weights as they are, scaled by 2^-40: with weights of up to 2^kRescaleLog2 a sum could pass the largest
+// fp32 although its mean does not. Rare, so plain: one tile at a time, no LDS.
+// One column block, so that few registers are needed beside the other blocks' sums.
+template <int DT, int D, int KT>
+__device__ __forceinline__ void careful_block(const TreeArgs& a, const Piece& p, Rows<D, 1>& rows, int wk, int lane) {
+  constexpr int KC = D / 32, MT = D / 16;
+  constexpr float kBias = 40.0f;
+  const int i16 = lane & 15, grp = lane >> 4;
+  const int32_t* table = a.bt + static_cast<int64_t>(p.s) * a.bt_stride;
+  rows.clear();
+  auto row_of = [&](int key, bool& ok) {
+    const int b = table[key >> a.log2_bs];
+    ok = b >= 0 && b < a.ncb;
+    return static_cast<uint64_t>(ok ? static_cast<uint32_t>(b) : 0u) * static_cast<uint32_t>(a.hkv * a.bs) +
+           static_cast<uint32_t>(p.kvh * a.bs + (key & (a.bs - 1)));
+  };
+#pragma unroll 1
+  for (int t = p.step0; t < p.step1; ++t) {
+    const int key0 = t * KT + wk * 32;
+    if (key0 > p.last) break;
+    bool ok;
+    const int mine = key0 + (lane & 31);
+    row_of(mine < p.last ? mine : p.last, ok);
+    const uint32_t real = static_cast<uint32_t>(__ballot(ok && mine <= p.last));
+    float sv[1][8];
+    {
+      u32x4_t k[2][KC];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int key = key0 + 16 * u + i16;
+        const char* row = a.k + row_of(key < p.last ? key : p.last, ok) * (2 * D) + 16 * grp;
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc) k[u][kc] = *reinterpret_cast<const u32x4_t*>(row + 64 * kc);
+      }
+      score_tile<DT, D, 1>(a, p, rows, k, key0, real, grp, sv);
+    }
+    const uint32_t win = rows.live[0] ? mask_window(a, p, rows.tok[0], key0) & real : 0u;
+    float pr[8];
+    weights(sv[0], rows.m[0] + kBias, a.scale_log2, pr);
+#pragma unroll 1
+    for (int kk = 0; kk < 32; ++kk) {
+      const int e = (kk & 3) + (kk >= 16 ? 4 : 0);
+      float pk = pr[0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) pk = e == i ? pr[i] : pk;
+      pk = __shfl(pk, ((kk & 15) >> 2) * 16 + i16);
+      if (!((real >> kk) & 1u)) continue;
+      const uint16_t* v = reinterpret_cast<const uint16_t*>(a.v + row_of(key0 + kk, ok) * (2 * D)) + 4 * grp;
+      if (!((win >> kk) & 1u)) continue;
+      rows.l[0] += pk;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) rows.acc[0][mt][i] += pk * widen<DT>(v[16 * mt + i]);
+    }
+  }
+  rows.m[0] += kBias;  // what the sums are relative to
+}
+
+template <int DT, int D, int NC, int KT>
+__device__ __forceinline__ void careful_pass(const TreeArgs& a, const Piece& p, Rows<D, NC>& rows, int first, int wk, int lane) {
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    Rows<D, 1> one;
+    one.load(a, p, first + 16 * c, lane & 15, lane >> 4);
+    careful_block<DT, D, KT>(a, p, one, wk, lane);
+    rows.m[c] = one.m[0];
+    rows.l[c] = one.l[0];
+#pragma unroll
+    for (int mt = 0; mt < D / 16; ++mt) rows.acc[c][mt] = one.acc[0][mt];
+  }
+}
+
+// Direct global -> LDS loads: 64 lanes x 16 bytes to l + 16 lane. K/V rows of a private pass are read once a call: the
+// nontemporal policy.
+typedef __attribute__((address_space(1))) void gvoid_t;
+typedef __attribute__((address_space(3))) void lvoid_t;
+typedef __attribute__((address_space(3))) char lchar_t;
+__device__ __forceinline__ void dma16(const char* g, lchar_t* l) {
+  __builtin_amdgcn_global_load_lds((gvoid_t*)g, (lvoid_t*)l, 16, 0, 2);
+}
+template <int N> __device__ __forceinline__ void wait_vmcnt() {
+  static_assert(N >= 0 && N < 64, "vmcnt field is 6 bits");
+  __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));  // no wait on the other counters
+}
+
+// LDS reads of a ring tile. They are asm because the compiler cannot tell which tile a direct load fills and would
+// drain every load before each read; each block waits for its own reads.
+template <int D> struct RingRead;
+template <> struct RingRead<64> {
+  static __device__ __forceinline__ void k(u32x4_t (&k)[2][2], const uint32_t (&at)[2]) {
+    asm volatile(
+        "ds_read_b128 %0, %4\n\tds_read_b128 %1, %5\n\tds_read_b128 %2, %4 offset:2048\n\t"
+        "ds_read_b128 %3, %5 offset:2048\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(k[0][0]), "=&v"(k[0][1]), "=&v"(k[1][0]), "=&v"(k[1][1])
+        : "v"(at[0]), "v"(at[1])
+        : "memory");
+  }
+};
+template <> struct RingRead<128> {
+  static __device__ __forceinline__ void k(u32x4_t (&k)[2][4], const uint32_t (&at)[4]) {
+    asm volatile(
+        "ds_read_b128 %0, %8\n\tds_read_b128 %1, %9\n\tds_read_b128 %2, %10\n\tds_read_b128 %3, %11\n\t"
+        "ds_read_b128 %4, %8 offset:4096\n\tds_read_b128 %5, %9 offset:4096\n\tds_read_b128 %6, %10 offset:4096\n\t"
+        "ds_read_b128 %7, %11 offset:4096\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(k[0][0]), "=&v"(k[0][1]), "=&v"(k[0][2]), "=&v"(k[0][3]), "=&v"(k[1][0]), "=&v"(k[1][1]),
+          "=&v"(k[1][2]), "=&v"(k[1][3])
+        : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3])
+        : "memory");
+  }
+};
+// V^T of four 16-dim tiles: rows 4 grp .. and 16 + 4 grp .. (HALF bytes on), transposed.
+template <int HALF>
+__device__ __forceinline__ void ring_v4(u32x2_t (&lo)[4], u32x2_t (&hi)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                        uint32_t a3) {
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %9\n\tds_read_b64_tr_b16 %2, %10\n\t"
+      "ds_read_b64_tr_b16 %3, %11\n\tds_read_b64_tr_b16 %4, %8 offset:%12\n\tds_read_b64_tr_b16 %5, %9 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %6, %10 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(lo[0]), "=&v"(lo[1]), "=&v"(lo[2]), "=&v"(lo[3]), "=&v"(hi[0]), "=&v"(hi[1]), "=&v"(hi[2]), "=&v"(hi[3])
+      : "v"(a0), "v"(a1), "v"(a2), "v"(a3), "i"(HALF)
+      : "memory");
+}
+
+// A wavefront's keys of a piece, fetched by itself: 32 of every step of 128. Direct loads fill its two LDS tiles of
+// K and V rows in turn, the next tile's while this one is computed, so loads in flight cost no registers and
+// wavefronts never wait for each other. Row r keeps its 16-byte chunk c at c ^ (r % CPR) (K) or c ^ vsw(r) (V), by the
+// choice of the chunk that each lane fetches.
+template <int DT, int D, int NC>
+__device__ __forceinline__ void private_pass(const TreeArgs& a, const Piece& p, Rows<D, NC>& rows, lchar_t* ring, int wk,
+                                             int lane) {
+  constexpr int KC = D / 32, MT = D / 16, RB = 2 * D, CPR = RB / 16, RPD = kWave / CPR, ND = 32 / RPD;
+  constexpr int TILE = 64 * RB, V_OFF = 32 * RB;
+  const int i16 = lane & 15, grp = lane >> 4;
+  const int32_t* table = a.bt + static_cast<int64_t>(p.s) * a.bt_stride;
+  const int last = p.last, ncb = static_cast<int>(a.ncb);
+  const uint32_t per_block = static_cast<uint32_t>(a.hkv * a.bs), head = static_cast<uint32_t>(p.kvh * a.bs);
+  rows.clear();
+  // Tiles of this wavefront: steps whose first key of its 32 exists.
+  const int mine = last < wk * 32 ? 0 : (last - wk * 32) / 128 + 1;
+  const int t1 = p.step1 < mine ? p.step1 : mine;
+  if (p.step0 >= t1) return;
+
+  const bool wide = a.bs >= 16;  // each half of a tile lies in one block, found by a scalar load
+  int id0 = 0, id1 = 0;          // of the tile that is fetched next
+  auto lookup = [&](int t) __attribute__((always_inline)) {
+    if (!wide) return;
+    const int key0 = t * 128 + wk * 32, key1 = key0 + 16 < last ? key0 + 16 : last;
+    id0 = load_uniform_i32(table + (key0 >> a.log2_bs));
+    id1 = load_uniform_i32(table + (key1 >> a.log2_bs));
+  };
+  // Start the loads of tile t into `to`; returns which of its keys exist and lie in the pool. Keys past the last one
+  // stand for it, block ids outside the pool for block 0.
+  auto fetch = [&](int t, lchar_t* to) __attribute__((always_inline)) -> uint32_t {
+    const int key0 = t * 128 + wk * 32;
+    uint32_t real = last - key0 >= 31 ? 0xffffffffu : (2u << (last - key0)) - 1u;
+    const bool ok0 = id0 >= 0 && id0 < ncb, ok1 = id1 >= 0 && id1 < ncb;
+    if (wide)
+      real &= (ok0 ? 0xffffu : 0u) | (ok1 ? 0xffff0000u : 0u);
+    else {
+      const int key = key0 + (lane & 31), b = table[(key < last ? key : last) >> a.log2_bs];
+      real &= static_cast<uint32_t>(__ballot(b >= 0 && b < ncb));
+    }
+#pragma unroll
+    for (int j = 0; j < ND; ++j) {
+      const int r = j * RPD + lane / CPR, c = lane % CPR;
+      const int key = key0 + r < last ? key0 + r : last;
+      int blk;
+      if (wide) {
+        blk = j * RPD < 16 ? (ok0 ? id0 : 0) : (ok1 ? id1 : 0);
+      } else {
+        blk = table[key >> a.log2_bs];
+        blk = blk >= 0 && blk < ncb ? blk : 0;
+      }
+      const uint64_t row = static_cast<uint64_t>(static_cast<uint32_t>(blk)) * per_block +
+                           (head + static_cast<uint32_t>(key & (a.bs - 1)));
+      dma16(a.k + row * RB + ((c ^ (r & (CPR - 1))) * 16), to + j * 1024);
+      dma16(a.v + row * RB + ((c ^ vsw<D>(r)) * 16), to + V_OFF + j * 1024);
+    }
+    return real;
+  };
+
+  uint32_t k_at[KC], v_at[MT];
+  const int vrow = 4 * grp + (i16 >> 2);  // rows vrow and vrow + 16 share vsw
+#pragma unroll
+  for (int kc = 0; kc < KC; ++kc)
+    k_at[kc] = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(ring)) + i16 * RB + (((4 * kc + grp) ^ (i16 & (CPR - 1))) * 16);
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+    v_at[mt] = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(ring)) + V_OFF + vrow * RB + (i16 & 3) * 8 +
+               (((2 * mt) ^ vsw<D>(vrow)) * 16);
+  lookup(p.step0);
+  uint32_t real = fetch(p.step0, ring), next = 0;
+  if (p.step0 + 1 < t1) lookup(p.step0 + 1);
+  uint32_t flip = 0;  // byte offset of the tile in use
+  for (int t = p.step0; t < t1; ++t) {
+    if (t + 1 < t1) {
+      next = fetch(t + 1, ring + (flip ^ TILE));
+      if (t + 2 < t1) lookup(t + 2);
+      wait_vmcnt<2 * ND>();
+    } else {
+      wait_vmcnt<0>();
+    }
+    u32x4_t k[2][KC];
+    uint32_t at[KC];
+#pragma unroll
+    for (int kc = 0; kc < KC; ++kc) at[kc] = k_at[kc] + flip;
+    RingRead<D>::k(k, at);
+    float sv[NC][8];
+    score_tile<DT, D, NC>(a, p, rows, k, t * 128 + wk * 32, real, grp, sv);
+    u32x4_t vt[MT];
+#pragma unroll
+    for (int q = 0; q < MT / 4; ++q) {
+      u32x2_t lo[4], hi[4];
+      ring_v4<16 * RB>(lo, hi, v_at[4 * q] + flip, v_at[4 * q + 1] + flip, v_at[4 * q + 2] + flip, v_at[4 * q + 3] + flip);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) vt[4 * q + i] = u32x4_t{lo[i][0], lo[i][1], hi[i][0], hi[i][1]};
+    }
+    value_tile<DT, D, NC>(rows, vt, sv, a.scale_log2);
+    real = next;
+    flip ^= TILE;
+  }
+}
+
+// A workgroup's keys of a piece, staged by all its threads for all its wavefronts: two LDS stages of a step, the
+// next step's rows in registers meanwhile. WR x WK wavefronts: WK take different 32 keys of a step. bf16 V is staged
+// as fp16, once for all rows.
+template <int DT, int D, int WR, int WK, int NC>
+__device__ __forceinline__ void shared_pass(const TreeArgs& a, const Piece& p, Rows<D, NC>& rows, char* smem, Shared& sh,
+                                            int w, int lane) {
+  using P = Shape<D, WR, WK, NC>;
+  constexpr int KC = P::KC, MT = P::MT, RB = P::RB, CPR = P::CPR, NLD = P::NLD;
+  const int tid = w * kWave + lane, wk = w % WK, i16 = lane & 15, grp = lane >> 4;
+  const int32_t* table = a.bt + static_cast<int64_t>(p.s) * a.bt_stride;
+  const int last = p.last;
+  rows.clear();
+  u32x4_t kbuf[NLD], vbuf[NLD];
+  bool okbuf = true;
   int bid[NLD];
   auto lookup = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
@@ -211,59 +563,33 @@ __device__ __forceinline__ bool run_piece(const TreeArgs& a, const Piece& p, int
     }
   };
   auto fetch = [&](int t) __attribute__((always_inline)) {
+    okbuf = true;
 #pragma unroll
     for (int j = 0; j < NLD; ++j) {
-      const int idx = tid + j * P::T;
-      const int r = idx / CPR, c = idx % CPR;
-      const int key = t * P::KT + r;
-      const int kk = key < last ? key : last;  // keys past the last one stand for it
+      const int idx = tid + j * P::T, r = idx / CPR, c = idx % CPR;
+      const int key = t * P::KT + r, kk = key < last ? key : last;  // keys past the last one stand for it
       const bool bok = bid[j] >= 0 && bid[j] < a.ncb;
       const uint64_t row = static_cast<uint64_t>(bok ? static_cast<uint32_t>(bid[j]) : 0u) *
                                static_cast<uint32_t>(a.hkv * a.bs) +
                            static_cast<uint32_t>(p.kvh * a.bs + (kk & (a.bs - 1)));
-      kbuf[j] = *reinterpret_cast<const uint4*>(a.k + row * RB + c * 16);
-      vbuf[j] = *reinterpret_cast<const uint4*>(a.v + row * RB + c * 16);
-      okbuf[j] = bok;
+      kbuf[j] = *reinterpret_cast<const u32x4_t*>(a.k + row * RB + c * 16);
+      vbuf[j] = *reinterpret_cast<const u32x4_t*>(a.v + row * RB + c * 16);
+      okbuf = okbuf && bok && key <= last;
     }
   };
   auto stash = [&](int stage) __attribute__((always_inline)) {
     char* st = smem + stage * P::STAGE;
-    bool ok = true, wild = false;
 #pragma unroll
     for (int j = 0; j < NLD; ++j) {
-      const int idx = tid + j * P::T;
-      const int r = idx / CPR, c = idx % CPR;
-      uint4 vv = vbuf[j];
-      if constexpr (VF16) vv = bf16x8_to_f16x8(vv);
-      if constexpr (CAREFUL)
-        vv = make_uint4(finite2<DT>(vv.x, wild), finite2<DT>(vv.y, wild), finite2<DT>(vv.z, wild), finite2<DT>(vv.w, wild));
-      *reinterpret_cast<uint4*>(st + r * RB + ((c ^ (r & (CPR - 1))) * 16)) = kbuf[j];
-      *reinterpret_cast<uint4*>(st + P::TILE + r * RB + ((c ^ P::vsw(r)) * 16)) = vv;
-      ok = ok && okbuf[j];
+      const int idx = tid + j * P::T, r = idx / CPR, c = idx % CPR;
+      u32x4_t vv = vbuf[j];
+      if constexpr (DT == MIP_BF16) vv = bf16x8_to_f16x8(vv);
+      *reinterpret_cast<u32x4_t*>(st + r * RB + ((c ^ (r & (CPR - 1))) * 16)) = kbuf[j];
+      *reinterpret_cast<u32x4_t*>(st + P::TILE + r * RB + ((c ^ vsw<D>(r)) * 16)) = vv;
     }
-    ok = __all(ok);
+    const bool ok = __all(okbuf);
     if (lane == 0) reinterpret_cast<uint8_t*>(&sh.ok[stage])[w] = ok ? 1 : 0;
-    if constexpr (CAREFUL) {
-      wild = __any(wild);
-      if (lane == 0) reinterpret_cast<uint8_t*>(&sh.wild[stage])[w] = wild ? 1 : 0;
-    }
   };
-  constexpr uint32_t kAllOk = P::NW == 4 ? 0x01010101u : P::NW == 2 ? 0x0101u : 0x01u;
-  static_assert(P::NW == 4 || P::NW == 2 || P::NW == 1, "one byte per wavefront");
-
-  f32x4_t acc[NC][MT];
-  f32x4_t lacc[NC];  // row sums by MFMA against a block of ones: every element holds row i16's
-  float m[NC], mth[NC], nm[NC];  // running maximum, the raw score that raises it, -m (0 while m = -inf)
-#pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    m[c] = -INFINITY;
-    mth[c] = -INFINITY;
-    nm[c] = 0.0f;
-    lacc[c] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) acc[c][mt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  }
-
   lookup(p.step0);
   fetch(p.step0);
   if (p.step0 + 1 < p.step1) lookup(p.step0 + 1);
@@ -278,396 +604,249 @@ __device__ __forceinline__ bool run_piece(const TreeArgs& a, const Piece& p, int
     const char* st = smem + stage * P::STAGE + wk * 32 * RB;
     const int key0 = t * P::KT + wk * 32;
     if (key0 <= last) {
-      uint4 kreg[2][KC];
+      u32x4_t k[2][KC];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
 #pragma unroll
         for (int kc = 0; kc < KC; ++kc) {
           const int r = 16 * u + i16, ch = 4 * kc + grp;
-          kreg[u][kc] = *reinterpret_cast<const uint4*>(st + r * RB + ((ch ^ (r & (CPR - 1))) * 16));
+          k[u][kc] = *reinterpret_cast<const u32x4_t*>(st + r * RB + ((ch ^ (r & (CPR - 1))) * 16));
         }
       }
-      // The PV product's k index 8 grp + i stands for key 4 grp + i (i < 4) or 16 + 4 grp + i - 4: the keys
-      // of this lane's two S^T halves.
-      uint4 vt[MT];
-      const int vrow = 4 * grp + (i16 >> 2), vs = P::vsw(vrow);  // rows vrow and vrow + 16 share vsw
-      const char* vb = st + P::TILE + vrow * RB + (i16 & 3) * 8;
+      u32x4_t vt[MT];
+      const int vrow = 4 * grp + (i16 >> 2), vs = vsw<D>(vrow);  // rows vrow and vrow + 16 share vsw
+      const char* vr = st + P::TILE + vrow * RB + (i16 & 3) * 8;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         const int so = ((2 * mt) ^ vs) * 16;
-        const uint2 lo = lds_tr16(vb + so);
-        const uint2 hi = lds_tr16(vb + 16 * RB + so);
-        vt[mt] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        const uint2 lo = lds_tr16(vr + so), hi = lds_tr16(vr + 16 * RB + so);
+        vt[mt] = u32x4_t{lo.x, lo.y, hi.x, hi.y};
       }
-      constexpr int kr[8] = {0, 1, 2, 3, 16, 17, 18, 19};  // this lane's keys: 4 grp + kr[i]
+      uint32_t real = 0xffffffffu;
+      if (__builtin_amdgcn_readfirstlane(sh.ok[stage]) != 0x01010101u) {  // the tile's keys one by one
+        const int key = key0 + (lane & 31);
+        const int b = table[(key < last ? key : last) >> a.log2_bs];
+        real = static_cast<uint32_t>(__ballot(key <= last && b >= 0 && b < a.ncb));
+      }
       float sv[NC][8];
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        f32x4_t s0 = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}, s1 = s0;
-#pragma unroll
-        for (int kc = 0; kc < KC; ++kc) {
-          s0 = Ops::qk(kreg[0][kc], qreg[c][kc], s0);
-          s1 = Ops::qk(kreg[1][kc], qreg[c][kc], s1);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sv[c][i] = i < 4 ? s0[i] : s1[i - 4];
-      }
-      const bool allok = __builtin_amdgcn_readfirstlane(sh.ok[stage]) == kAllOk;
-      uint32_t win[NC];  // bit k: this lane's row sees key key0 + k
-      const bool open = allok && key0 + 31 < p.ctx && key0 + 31 <= last;  // cached keys only: everybody sees them
-      if (!open) {
-        const int e0 = key0 - p.ctx;  // tree number of the first key (below 0: cached)
-        uint32_t real = last - key0 >= 31 ? 0xffffffffu : (2u << (last - key0)) - 1u;
-        if (!allok) {  // blocks outside the pool: the tile's keys one by one
-          const int key = key0 + (lane & 31);
-          const int b = table[(key < last ? key : last) >> a.log2_bs];
-          real &= static_cast<uint32_t>(__ballot(b >= 0 && b < a.ncb));
-        }
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          uint32_t see = 0xffffffffu;
-          if (e0 > -32) {
-            const uint64_t* row = a.mask + (static_cast<int64_t>(p.q0) + tok[c]) * a.mask_st;
-            if (e0 < 0) {
-              see = static_cast<uint32_t>(row[0] << -e0) | ((1u << -e0) - 1u);
-            } else {
-              const int word = e0 >> 6, off = e0 & 63;
-              uint64_t x = word < a.mask_words ? row[word] >> off : 0;
-              if (off > 32 && word + 1 < a.mask_words) x |= row[word + 1] << (64 - off);
-              see = static_cast<uint32_t>(x);
-            }
-          }
-          win[c] = live[c] ? see & real : 0u;
-          const uint32_t mine = win[c] >> (4 * grp);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) sv[c][i] = (mine >> kr[i]) & 1u ? sv[c][i] : -INFINITY;
-        }
-      } else {
-#pragma unroll
-        for (int c = 0; c < NC; ++c) win[c] = 0xffffffffu;
-      }
-      float mx[NC];
-      bool need = false;
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        mx[c] = fmax3(fmax3(sv[c][0], sv[c][1], sv[c][2]), fmax3(sv[c][3], sv[c][4], sv[c][5]),
-                      fmax2(sv[c][6], sv[c][7]));
-        need = need || mx[c] > mth[c];
-      }
-      if (__any(need)) {
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          if (__any(mx[c] > mth[c])) {
-            const float mn = fmax2(m[c], max4(mx[c]) * a.scale_log2);
-            const float alpha = (m[c] == -INFINITY) ? 0.0f : fast_exp2(m[c] - mn);
-            lacc[c] *= alpha;
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) acc[c][mt] *= alpha;
-            m[c] = mn;
-            mth[c] = (mn + kRescaleLog2) / a.scale_log2;
-            nm[c] = mn == -INFINITY ? 0.0f : -mn;
-          }
-        }
-      }
-      const bool wild = CAREFUL && __builtin_amdgcn_readfirstlane(sh.wild[stage]) != 0;
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        float pr[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) pr[i] = fast_exp2(fmaf(sv[c][i], a.scale_log2, nm[c]));
-        uint4 ph;
-        ph.x = OpsV::pack2(pr[0], pr[1]);
-        ph.y = OpsV::pack2(pr[2], pr[3]);
-        ph.z = OpsV::pack2(pr[4], pr[5]);
-        ph.w = OpsV::pack2(pr[6], pr[7]);
-        constexpr uint32_t kOne2 = DT == MIP_BF16 && !VF16 ? 0x3f803f80u : 0x3c003c00u;
-        const uint4 ones = make_uint4(kOne2, kOne2, kOne2, kOne2);
-        lacc[c] = OpsV::qk(ones, ph, lacc[c]);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) acc[c][mt] = OpsV::qk(vt[mt], ph, acc[c][mt]);
-        if constexpr (CAREFUL) {
-          uint4 pl;
-          pl.x = Ops::pack2(pr[0] - Ops::lo(ph.x), pr[1] - Ops::hi(ph.x));
-          pl.y = Ops::pack2(pr[2] - Ops::lo(ph.y), pr[3] - Ops::hi(ph.y));
-          pl.z = Ops::pack2(pr[4] - Ops::lo(ph.z), pr[5] - Ops::hi(ph.z));
-          pl.w = Ops::pack2(pr[6] - Ops::lo(ph.w), pr[7] - Ops::hi(ph.w));
-          lacc[c] = Ops::qk(ones, pl, lacc[c]);
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) acc[c][mt] = Ops::qk(vt[mt], pl, acc[c][mt]);
-          if (wild) {
-            // Values that are inf or NaN were staged as 0: each joins the rows that see its key.
-#pragma unroll 1
-            for (int kk = 0; kk < 32 && key0 + kk <= last; ++kk) {
-              const int e = (kk & 3) + (kk >= 16 ? 4 : 0);
-              float pk = pr[0];
-#pragma unroll
-              for (int i = 1; i < 8; ++i) pk = e == i ? pr[i] : pk;
-              pk = __shfl(pk, ((kk & 15) >> 2) * 16 + i16);
-              const int b = table[(key0 + kk) >> a.log2_bs];
-              if (b < 0 || b >= a.ncb) continue;
-              const uint64_t row = static_cast<uint64_t>(b) * static_cast<uint32_t>(a.hkv * a.bs) +
-                                   static_cast<uint32_t>(p.kvh * a.bs + ((key0 + kk) & (a.bs - 1)));
-              const uint16_t* vr = reinterpret_cast<const uint16_t*>(a.v + row * RB);
-              const bool seen = (win[c] >> kk) & 1u;
-#pragma unroll
-              for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const float x = widen<DT>(vr[16 * mt + 4 * grp + i]);
-                  if (seen && !(fabsf(x) < INFINITY)) acc[c][mt][i] += pk * x;
-                }
-            }
-          }
-        }
-      }
+      score_tile<DT, D, NC>(a, p, rows, k, key0, real, grp, sv);
+      value_tile<MIP_F16, D, NC>(rows, vt, sv, a.scale_log2);
     }
     if (t + 1 < p.step1) stash(stage ^ 1);
     __syncthreads();
   }
-
-  // ---- a fast pass that met inf or NaN runs again. Every thread reads the flag before any writes it again.
-  if constexpr (!CAREFUL) {
-    float big = 0.0f;
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-        big = fmax3(big, fmax2(fabsf(acc[c][mt][0]), fabsf(acc[c][mt][1])),
-                    fmax2(fabsf(acc[c][mt][2]), fabsf(acc[c][mt][3])));
-    if (__any(!(big < INFINITY)) && lane == 0) sh.tag = tag;
-    __syncthreads();
-    const bool again = __builtin_amdgcn_readfirstlane(sh.tag) == tag;
-    __syncthreads();
-    if (again) return true;
-  }
-
-  // ---- the wavefronts of one row block meet: wavefront wk = 0 takes the others' sums.
-  if constexpr (WK > 1) {
-    f32x4_t* park = reinterpret_cast<f32x4_t*>(smem);
-    if (wk > 0) {
-      const int at = wr * (WK - 1) + wk - 1;
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) park[((at * NC + c) * MT + mt) * kWave + lane] = acc[c][mt];
-        if (grp == 0) {
-          sh.ml[0][(at * NC + c) * 16 + i16] = m[c];
-          sh.ml[1][(at * NC + c) * 16 + i16] = lacc[c][0];
-        }
-      }
-    }
-    __syncthreads();
-    if (wk == 0) {
-#pragma unroll
-      for (int o = 0; o < WK - 1; ++o) {
-        const int at = wr * (WK - 1) + o;
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          const float mo = sh.ml[0][(at * NC + c) * 16 + i16], lo = sh.ml[1][(at * NC + c) * 16 + i16];
-          const float mn = fmax2(m[c], mo);
-          // A part without keys has sums of 0 (its maximum is -inf, and so may both be).
-          const float fa = m[c] == -INFINITY ? 0.0f : fast_exp2(m[c] - mn);
-          const float fb = mo == -INFINITY ? 0.0f : fast_exp2(mo - mn);
-          m[c] = mn;
-          lacc[c][0] = lacc[c][0] * fa + lo * fb;
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            const f32x4_t x = park[((at * NC + c) * MT + mt) * kWave + lane];
-            acc[c][mt] = acc[c][mt] * fa + x * fb;
-          }
-        }
-      }
-    }
-  }
-
-  if (wk == 0) {
-    if (rec >= 0) {
-      // Record: accumulators as the lanes hold them, [column block][mt][lane].
-      float* base = a.ws_rec + rec * a.rec_floats;
-      f32x4_t* racc = reinterpret_cast<f32x4_t*>(base + 2 * P::R);
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const int cb = wr * NC + c;
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) racc[(cb * MT + mt) * kWave + lane] = acc[c][mt];
-        if (grp == 0) {
-          base[cb * 16 + i16] = m[c];
-          base[P::R + cb * 16 + i16] = lacc[c][0];
-        }
-      }
-    } else {
-      using S = typename Elem<DT>::S;
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        if (!live[c]) continue;
-        const float lt = lacc[c][0];
-        const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;  // 0: no key seen, sums of 0
-        const int r = p.rb * P::R + (wr * NC + c) * 16 + i16;
-        S* orow = reinterpret_cast<S*>(a.out) + (static_cast<int64_t>(p.q0) + tok[c]) * a.out_st +
-                  static_cast<int64_t>(p.kvh * G + r - tok[c] * G) * a.out_sh;
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          const uint32_t w0 = Ops::pack2(acc[c][mt][0] * inv, acc[c][mt][1] * inv);
-          const uint32_t w1 = Ops::pack2(acc[c][mt][2] * inv, acc[c][mt][3] * inv);
-          *reinterpret_cast<uint2*>(orow + 16 * mt + 4 * grp) = make_uint2(w0, w1);
-        }
-      }
-    }
-  }
-  if constexpr (WK > 1) __syncthreads();  // the next piece stages over the parked sums
-  return false;
 }
 
-template <int DT, int D, int WR, int WK, int NC>
-__global__ __launch_bounds__(WR * WK * kWave) __attribute__((amdgpu_waves_per_eu(WR * WK / 2, WR * WK / 2)))
-void paged_tree_kernel(TreeArgs a) {
-  using P = Shape<D, WR, WK, NC>;
-  constexpr int T = P::T, NW = P::NW, ML = WK > 1 ? WR * (WK - 1) * NC * 16 : 1;
-  __shared__ __attribute__((aligned(16))) char smem[2 * P::STAGE];
-  __shared__ Shared<T, NW, ML> sh;
-  const int tid = threadIdx.x, lane = tid & (kWave - 1), w = tid / kWave;
-  const int S = a.num_seqs, cap = a.max_blocks * a.bs;
-
-  // ---- steps of all segments, then the piece length L, then every sequence's first piece and record.
-  auto segments = [&](const Piece& p) { return (p.n * a.group + P::R - 1) / P::R * a.hkv; };
-  auto steps = [&](const Piece& p) { return (p.keys + P::KT - 1) / P::KT; };
-  int sum = 0;
-  for (int s = tid; s < S; s += T) {
-    const Piece p = seq_shape(a, s, cap);
-    sum += segments(p) * steps(p);
-  }
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) sum += __shfl_xor(sum, d);
-  if (lane == 0) sh.scan[0][w] = sum;
-  if (tid == 0) {
-    sh.tag = 0;
-    sh.ok[0] = sh.ok[1] = sh.wild[0] = sh.wild[1] = 0;
-  }
-  __syncthreads();
-  int total = 0;
-#pragma unroll
-  for (int i = 0; i < NW; ++i) total += sh.scan[0][i];
-  __syncthreads();
-  int L = (total + a.target - 1) / a.target;
-  L = L > a.min_steps ? L : a.min_steps;
-  int base_p = 0, base_r = 0;
-  for (int s0 = 0; s0 < S; s0 += T) {
-    const int s = s0 + tid;
-    int np = 0, nr = 0;
-    if (s < S) {
-      const Piece p = seq_shape(a, s, cap);
-      const int cuts = (steps(p) + L - 1) / L, segs = segments(p);
-      np = segs * cuts;
-      nr = cuts > 1 ? np : 0;
-    }
-    const int ip = decode::wave_inclusive_scan(np, lane), ir = decode::wave_inclusive_scan(nr, lane);
-    if (lane == kWave - 1) {
-      sh.scan[0][w] = ip;
-      sh.scan[1][w] = ir;
-    }
-    __syncthreads();
-    int before_p = base_p, before_r = base_r;
-#pragma unroll
-    for (int i = 0; i < NW; ++i) {
-      if (i < w) {
-        before_p += sh.scan[0][i];
-        before_r += sh.scan[1][i];
-      }
-      base_p += sh.scan[0][i];
-      base_r += sh.scan[1][i];
-    }
-    if (s < S) {
-      sh.pieces[s] = before_p + ip - np;
-      sh.recs[s] = before_r + ir - nr;
-    }
-    __syncthreads();
-  }
-  // Descriptors of records that no piece of this call has.
-  if (blockIdx.x == 0)
-    for (int i = base_r + tid; i < a.max_recs; i += T) a.ws_desc[i * kDesc] = 0;
-
-  // ---- pieces, each XCD a contiguous range of them (row blocks of the same keys are neighbours and meet in
-  // its L2).
-  const int per_xcd = (base_p + 7) / 8, xcd = blockIdx.x & 7;
-  const int stride = static_cast<int>(gridDim.x) / 8;
-  for (int i = blockIdx.x >> 3; i < per_xcd; i += stride) {
-    const int it = xcd * per_xcd + i;
-    if (it >= base_p) break;
-    int lo = 0, hi = S - 1;  // the last sequence with pieces[s] <= it (those before it without pieces are passed by)
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (sh.pieces[mid] <= it) lo = mid; else hi = mid - 1;
-    }
-    const int s = __builtin_amdgcn_readfirstlane(lo);
-    Piece p = seq_shape(a, s, cap);
-    const int nt = steps(p), cuts = (nt + L - 1) / L, nrb = (p.n * a.group + P::R - 1) / P::R;
-    const int at = __builtin_amdgcn_readfirstlane(it - sh.pieces[s]);  // ((kv head, piece), row block)
-    p.rb = at % nrb;
-    const int kj = at / nrb;
-    p.kvh = kj / cuts;
-    const int j = kj - p.kvh * cuts;
-    p.step0 = static_cast<int>(static_cast<int64_t>(nt) * j / cuts);
-    p.step1 = static_cast<int>(static_cast<int64_t>(nt) * (j + 1) / cuts);
-    int64_t rec = -1;
-    if (cuts > 1) {
-      const int first = __builtin_amdgcn_readfirstlane(sh.recs[s]) + (p.kvh * nrb + p.rb) * cuts;
-      rec = first + j;
-      if (tid == 0) {
-        int32_t* d = a.ws_desc + rec * kDesc;
-        d[0] = j == 0 ? cuts : 0;
-        d[1] = s;
-        d[2] = p.kvh;
-        d[3] = p.rb;
-      }
-    }
-    if (run_piece<DT, D, WR, WK, NC, false>(a, p, rec, it + 1u, smem, sh))
-      run_piece<DT, D, WR, WK, NC, true>(a, p, rec, it + 1u, smem, sh);
-  }
-}
-
-// Combine the pieces of every split segment. Workgroup (g, y): column block y of the segment whose first
-// record is g.
-template <int DT, int D, int R>
-__global__ __launch_bounds__(256) void paged_tree_merge(TreeArgs a) {
+// Output rows of a column block, or its part of a record (accumulators as the lanes hold them, [block][mt][lane]).
+template <int DT, int D, int R, int N>
+__device__ __forceinline__ void put_block(const TreeArgs& a, const Piece& p, float* rec, int cb, int mt0, bool live, int tok,
+                                          float m, float l, const f32x4_t (&acc)[N], int lane) {
   using Ops = MfmaOps<DT>;
   using S = typename Elem<DT>::S;
-  constexpr int MT = D / 16, PER = MT / 4;  // dim tiles; of each wavefront
-  const int g = blockIdx.x, cb = blockIdx.y;
-  const int32_t* d = a.ws_desc + g * kDesc;
-  const int pieces = d[0];
-  if (pieces == 0) return;
-  const int s = d[1], kvh = d[2], rb = d[3];
-  const int q0 = a.cu_q[s];
-  int n = a.cu_q[s + 1] - q0;
-  n = n < a.max_q_len ? n : a.max_q_len;
-  const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave, i16 = lane & 15, grp = lane >> 4;
-  const int r = rb * R + cb * 16 + i16, t = r / a.group, h = kvh * a.group + r - t * a.group;
-  if (rb * R + cb * 16 >= n * a.group) return;
-  const float* first = a.ws_rec + static_cast<int64_t>(g) * a.rec_floats;
+  const int i16 = lane & 15, grp = lane >> 4;
+  if (rec) {
+    f32x4_t* out = reinterpret_cast<f32x4_t*>(rec + 2 * R) + (cb * (D / 16) + mt0) * kWave + lane;
+#pragma unroll
+    for (int x = 0; x < N; ++x) out[x * kWave] = acc[x];
+    if (mt0 == 0 && grp == 0) {
+      rec[cb * 16 + i16] = m;
+      rec[R + cb * 16 + i16] = l;
+    }
+    return;
+  }
+  if (!live) return;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // 0: no key seen, sums of 0
+  const int r = p.rb * R + cb * 16 + i16;
+  S* row = reinterpret_cast<S*>(a.out) + (static_cast<int64_t>(p.q.q0) + tok) * a.out_st +
+           static_cast<int64_t>(p.kvh * a.group + r - tok * a.group) * a.out_sh;
+#pragma unroll
+  for (int x = 0; x < N; ++x) {
+    const uint32_t w0 = Ops::pack2(acc[x][0] * inv, acc[x][1] * inv), w1 = Ops::pack2(acc[x][2] * inv, acc[x][3] * inv);
+    *reinterpret_cast<uint2*>(row + 16 * (mt0 + x) + 4 * grp) = make_uint2(w0, w1);
+  }
+}
+
+// One piece: rows of block p.rb against steps [p.step0, p.step1). rec: null where that is the whole segment.
+template <int DT, int D, int WR, int WK, int NC>
+__device__ __forceinline__ void run_piece(const TreeArgs& a, const Piece& p, float* rec, char* smem, Shared& sh,
+                                          float (*sh_ml)[4][16 * NC]) {
+  using P = Shape<D, WR, WK, NC>;
+  constexpr int MT = P::MT;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int wr = w / WK, wk = w % WK, i16 = lane & 15, grp = lane >> 4;
+  Rows<D, NC> rows;
+  const int first = p.rb * P::R + wr * NC * 16;
+  rows.load(a, p, first, i16, grp);
+  if constexpr (P::kPrivate)
+    private_pass<DT, D, NC>(a, p, rows, (lchar_t*)(smem + w * P::kRing), wk, lane);
+  else
+    shared_pass<DT, D, WR, WK, NC>(a, p, rows, smem, sh, w, lane);
+  // A wavefront whose accumulators hold inf or NaN does its part again.
+  if (!rows.finite()) careful_pass<DT, D, NC, P::KT>(a, p, rows, first, wk, lane);
+  if constexpr (WK == 1) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      put_block<DT, D, P::R, MT>(a, p, rec, wr * NC + c, 0, rows.live[c], rows.tok[c], rows.m[c], rows.l[c][0], rows.acc[c],
+                                 lane);
+  } else {
+    // The WK wavefronts of a row meet: each scales its sums to the common maximum, and each takes MT / WK of
+    // the dims of every column block, which go through LDS one block at a time.
+    constexpr int PER = MT / WK;
+    if (grp == 0) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        sh_ml[0][w][c * 16 + i16] = rows.m[c];
+        sh_ml[1][w][c * 16 + i16] = rows.l[c][0];
+      }
+    }
+    __syncthreads();  // also: every wavefront is done with its stage
+    f32x4_t* park = reinterpret_cast<f32x4_t*>(smem);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      float m = -INFINITY, l = 0.0f;
+#pragma unroll
+      for (int o = 0; o < WK; ++o) m = fmax2(m, sh_ml[0][wr * WK + o][c * 16 + i16]);
+#pragma unroll
+      for (int o = 0; o < WK; ++o) {
+        const float mo = sh_ml[0][wr * WK + o][c * 16 + i16];
+        // A wavefront without keys has sums of 0 and a maximum of -inf (and so may all).
+        l += sh_ml[1][wr * WK + o][c * 16 + i16] * (mo == -INFINITY ? 0.0f : fast_exp2(mo - m));
+      }
+      const float f = rows.m[c] == -INFINITY ? 0.0f : fast_exp2(rows.m[c] - m);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) park[(w * MT + mt) * kWave + lane] = rows.acc[c][mt] * f;
+      __syncthreads();
+      f32x4_t sum[PER];
+#pragma unroll
+      for (int x = 0; x < PER; ++x) {
+        sum[x] = park[((wr * WK) * MT + wk * PER + x) * kWave + lane];
+#pragma unroll
+        for (int o = 1; o < WK; ++o) sum[x] += park[((wr * WK + o) * MT + wk * PER + x) * kWave + lane];
+      }
+      put_block<DT, D, P::R, PER>(a, p, rec, wr * NC + c, wk * PER, rows.live[c], rows.tok[c], m, l, sum, lane);
+      __syncthreads();
+    }
+  }
+}
+
+__device__ __forceinline__ int segments_of(const TreeArgs& a, const Seq& q, int rows) {
+  return (q.n * a.group + rows - 1) / rows * a.hkv;
+}
+
+template <int DT, int D, int WR, int WK, int NC, int OCC>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC))) void paged_tree_kernel(TreeArgs a) {
+  using P = Shape<D, WR, WK, NC>;
+  __shared__ __attribute__((aligned(16))) char smem[P::kLds];
+  __shared__ Shared sh;
+  __shared__ float sh_ml[2][4][16 * NC];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), w = tid / kWave;
+  const int S = a.num_seqs;
+  auto steps_of = [&](const Seq& q) { return (keys_of(a, q) + P::KT - 1) / P::KT; };
+
+  // ---- the place of every sequence's steps in the call's one row of steps.
+  int total = 0;
+  for (int s0 = 0; s0 < S; s0 += P::T) {
+    const int s = s0 + tid;
+    int n = 0;
+    if (s < S) {
+      const Seq q = seq_of(a, s);
+      n = segments_of(a, q, P::R) * steps_of(q);
+    }
+    const int incl = decode::wave_inclusive_scan(n, lane);
+    if (lane == kWave - 1) sh.scan[w] = incl;
+    __syncthreads();
+    int before = total;
+#pragma unroll
+    for (int i = 0; i < P::NW; ++i) {
+      before += i < w ? sh.scan[i] : 0;
+      total += sh.scan[i];
+    }
+    if (s < S) sh.start[s] = before + incl - n;
+    __syncthreads();
+  }
+
+  // ---- equal shares: worker i takes steps [i * share, i * share + share). The workers of an XCD are neighbours, so
+  // that row blocks of the same keys meet in its L2.
+  int share = (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+  share = share > a.min_share ? share : a.min_share;
+  const int workers = (total + share - 1) / share, per_xcd = (workers + 7) / 8;
+  const int worker = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+  if (a.ws_start && blockIdx.x == 0) {  // for the second kernel
+    for (int s = tid; s < S; s += P::T) a.ws_start[s] = sh.start[s];
+    if (tid == 0) a.ws_start[S] = share;
+  }
+  if (static_cast<int>(blockIdx.x >> 3) >= per_xcd || worker >= workers) return;
+  int at = worker * share;
+  const int end = at + share < total ? at + share : total;
+  int lo = 0, hi = S - 1;  // the last sequence that starts at or before `at`
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (sh.start[mid] <= at) lo = mid; else hi = mid - 1;
+  }
+  for (int s = lo; at < end; ++s) {
+    Piece p;
+    p.s = __builtin_amdgcn_readfirstlane(s);
+    p.q = seq_of(a, p.s);
+    p.last = keys_of(a, p.q) - 1;
+    const int nt = steps_of(p.q), segs = segments_of(a, p.q, P::R), nrb = segs / a.hkv;
+    const int first = __builtin_amdgcn_readfirstlane(sh.start[s]);
+    while (at < end && at < first + segs * nt) {
+      const int seg = (at - first) / nt, seg0 = first + seg * nt;
+      p.kvh = seg / nrb;
+      p.rb = seg - p.kvh * nrb;
+      p.step0 = at - seg0;
+      p.step1 = end - seg0 < nt ? end - seg0 : nt;
+      float* rec = nullptr;
+      // A worker's first piece, if it begins inside its segment, has record 0, its last, if it ends inside, 1.
+      if (p.step0 > 0 || p.step1 < nt)
+        rec = a.ws_rec + (static_cast<int64_t>(worker) * 2 + (p.step0 > 0 ? 0 : 1)) * P::kRec;
+      run_piece<DT, D, WR, WK, NC>(a, p, rec, smem, sh, sh_ml);
+      at = seg0 + p.step1;
+    }
+  }
+}
+
+// Combine the pieces of a split segment. Workgroup (x, cb): column block cb of segment x = (sequence, (kv head, row block));
+// each wavefront a quarter of the dims.
+template <int DT, int D, int R>
+__global__ __launch_bounds__(256) void paged_tree_merge(TreeArgs a, int segs_per_seq, int keys_per_step) {
+  constexpr int MT = D / 16, PER = MT / 4;
+  const int s = blockIdx.x / segs_per_seq, seg = blockIdx.x - s * segs_per_seq, cb = blockIdx.y;
+  Piece p;
+  p.s = s;
+  p.q = seq_of(a, s);
+  const int first = a.ws_start[s], share = a.ws_start[a.num_seqs];
+  const int nt = (keys_of(a, p.q) + keys_per_step - 1) / keys_per_step, segs = segments_of(a, p.q, R), nrb = segs / a.hkv;
+  if (seg >= segs) return;
+  const int begin = first + seg * nt, w0 = begin / share, w1 = (begin + nt - 1) / share;
+  if (w0 == w1) return;
+  p.kvh = seg / nrb;
+  p.rb = seg - p.kvh * nrb;
+  const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave, i16 = lane & 15;
+  if (p.rb * R + cb * 16 >= p.q.n * a.group) return;
+  constexpr int64_t kRec = 2 * R + static_cast<int64_t>(R) * D;
+  // The segment's first piece ends inside it (record 1 of its worker); the others begin inside it (record 0).
+  auto record = [&](int x) { return a.ws_rec + (static_cast<int64_t>(x) * 2 + (x == w0 ? 1 : 0)) * kRec; };
   float m = -INFINITY;
-  for (int p = 0; p < pieces; ++p) m = fmaxf(m, first[p * a.rec_floats + cb * 16 + i16]);
+#pragma unroll 4
+  for (int x = w0; x <= w1; ++x) m = fmax2(m, record(x)[cb * 16 + i16]);
   float l = 0.0f;
   f32x4_t acc[PER];
 #pragma unroll
-  for (int x = 0; x < PER; ++x) acc[x] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int i = 0; i < PER; ++i) acc[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-  for (int p = 0; p < pieces; ++p) {
-    const float* rec = first + p * a.rec_floats;
+  for (int x = w0; x <= w1; ++x) {
+    const float* rec = record(x);
     const float mp = rec[cb * 16 + i16];
     const float f = mp == -INFINITY ? 0.0f : fast_exp2(mp - m);
     l += f * rec[R + cb * 16 + i16];
     const f32x4_t* racc = reinterpret_cast<const f32x4_t*>(rec + 2 * R) + (cb * MT + w * PER) * kWave + lane;
 #pragma unroll
-    for (int x = 0; x < PER; ++x) acc[x] += racc[x * kWave] * f;
+    for (int i = 0; i < PER; ++i) acc[i] += racc[i * kWave] * f;
   }
-  if (t >= n) return;
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  S* orow = reinterpret_cast<S*>(a.out) + (static_cast<int64_t>(q0) + t) * a.out_st + static_cast<int64_t>(h) * a.out_sh;
-#pragma unroll
-  for (int x = 0; x < PER; ++x) {
-    const uint32_t w0 = Ops::pack2(acc[x][0] * inv, acc[x][1] * inv), w1 = Ops::pack2(acc[x][2] * inv, acc[x][3] * inv);
-    *reinterpret_cast<uint2*>(orow + 16 * (w * PER + x) + 4 * grp) = make_uint2(w0, w1);
-  }
+  const int r = p.rb * R + cb * 16 + i16, tok = r / a.group;
+  put_block<DT, D, R, PER>(a, p, nullptr, cb, w * PER, tok < p.q.n, tok, m, l, acc, lane);
 }
 
 // ------------------------------------------------------------------ one query row at a time
@@ -687,8 +866,9 @@ __global__ __launch_bounds__(256) void paged_tree_row_kernel(TreeArgs a, int hq)
   __shared__ float s_acc[kStates][D];
   const int64_t x = blockIdx.x;  // (sequence, node)
   const int s = static_cast<int>(x / a.max_q_len), i = static_cast<int>(x - static_cast<int64_t>(s) * a.max_q_len);
-  const Piece p = seq_shape(a, s, a.max_blocks * a.bs);
+  const Seq p = seq_of(a, s);
   if (i >= p.n) return;
+  const int keys = keys_of(a, p);
   const int h = blockIdx.y, kvh = h / a.group;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), w = tid / kWave;
   const int row = lane / LPR, c = lane % LPR;
@@ -710,9 +890,9 @@ __global__ __launch_bounds__(256) void paged_tree_row_kernel(TreeArgs a, int hq)
 #pragma unroll
     for (int e = 0; e < N; ++e) v[e] = widen<DT>(raw[e]);
   };
-  for (int base = 0; base < p.keys; base += 4 * RPP) {
+  for (int base = 0; base < keys; base += 4 * RPP) {
     const int key = base + w * RPP + row, e0 = key - p.ctx;
-    bool seen = key < p.keys;
+    bool seen = key < keys;
     if (seen && e0 >= 0) seen = (e0 >> 6) < a.mask_words && ((mask[e0 >> 6] >> (e0 & 63)) & 1u);
     const int blk = seen ? table[key >> a.log2_bs] : -1;
     seen = blk >= 0 && blk < a.ncb;
@@ -761,37 +941,38 @@ __global__ __launch_bounds__(256) void paged_tree_row_kernel(TreeArgs a, int hq)
 // ------------------------------------------------------------------ host side
 
 using KernelFn = void (*)(TreeArgs);
+using MergeFn = void (*)(TreeArgs, int, int);
 
 struct Config {
-  KernelFn fn = nullptr, merge = nullptr;
-  int rows = 0, keys = 0, threads = 0;  // R, KT
+  KernelFn fn = nullptr;
+  MergeFn merge = nullptr;
+  int rows = 0, keys = 0, occ = 0;  // R, KT, workgroups per CU
   int64_t rec_floats = 0;
 };
 
-template <int DT, int D, int WR, int WK, int NC>
+template <int DT, int D, int WR, int WK, int NC, int OCC>
 Config config_of() {
   using P = Shape<D, WR, WK, NC>;
-  return {paged_tree_kernel<DT, D, WR, WK, NC>, paged_tree_merge<DT, D, P::R>, P::R, P::KT, P::T, P::kRec};
+  return {paged_tree_kernel<DT, D, WR, WK, NC, OCC>, paged_tree_merge<DT, D, P::R>, P::R, P::KT, OCC, P::kRec};
 }
 
 // The workgroup's shape by the most rows a sequence can have.
 template <int DT>
 Config pick(int d, int64_t rows) {
   if (d == 64) {
-    if (rows <= 16) return config_of<DT, 64, 1, 4, 1>();
-    if (rows <= 32) return config_of<DT, 64, 1, 4, 2>();
-    if (rows <= 64) return config_of<DT, 64, 1, 4, 4>();
-    if (rows <= 128) return config_of<DT, 64, 2, 2, 4>();
-    return config_of<DT, 64, 4, 1, 4>();
+    if (rows <= 16) return config_of<DT, 64, 1, 4, 1, 2>();
+    if (rows <= 32) return config_of<DT, 64, 1, 4, 2, 2>();
+    if (rows <= 64) return config_of<DT, 64, 1, 4, 4, 2>();
+    if (rows <= 128) return config_of<DT, 64, 2, 2, 4, 2>();
+    return config_of<DT, 64, 4, 1, 4, 2>();
   }
-  if (rows <= 16) return config_of<DT, 128, 1, 2, 1>();
-  if (rows <= 32) return config_of<DT, 128, 1, 2, 2>();
-  if (rows <= 64) return config_of<DT, 128, 2, 2, 2>();
-  return config_of<DT, 128, 4, 1, 2>();
+  if (rows <= 16) return config_of<DT, 128, 1, 4, 1, 1>();
+  if (rows <= 32) return config_of<DT, 128, 1, 4, 2, 1>();
+  if (rows <= 64) return config_of<DT, 128, 1, 4, 4, 1>();
+  return config_of<DT, 128, 4, 1, 2, 2>();
 }
 
-constexpr int kWgPerCu = 2;
-constexpr int kMinSteps = 2;
+constexpr int kMinShareKeys = 256;  // fewest keys a worker takes
 
 int compute_units() {
   int dev = 0, cus = 0;
@@ -803,8 +984,8 @@ int compute_units() {
 struct Plan {
   Config cfg;
   bool ok = false;      // the matrix-core kernel takes this shape
-  int target = 0, grid = 0, max_recs = 0, rec_grid = 0;
-  int64_t desc_off = 0, bytes = 0;
+  int grid = 0, segs_per_seq = 0, min_share = 0;
+  int64_t start_off = 0, bytes = 0;  // bytes 0: no segment can be split
 };
 
 Plan plan_of(int num_seqs, int max_q_len, int hq, int hkv, int d, int bs, int max_blocks, int dtype) {
@@ -813,21 +994,21 @@ Plan plan_of(int num_seqs, int max_q_len, int hq, int hkv, int d, int bs, int ma
   const int64_t rows = static_cast<int64_t>(max_q_len) * group, cap = static_cast<int64_t>(max_blocks) * bs;
   if ((dtype != MIP_F16 && dtype != MIP_BF16) || (d != 64 && d != 128) || num_seqs > kMaxSeqs) return p;
   p.cfg = dtype == MIP_F16 ? pick<MIP_F16>(d, rows) : pick<MIP_BF16>(d, rows);
-  const int64_t segs = static_cast<int64_t>(num_seqs) * hkv * ((rows + p.cfg.rows - 1) / p.cfg.rows);
-  const int64_t steps = (cap + p.cfg.keys - 1) / p.cfg.keys;
-  if (segs * steps >= (int64_t{1} << 30)) return p;
+  const int64_t segs = hkv * ((rows + p.cfg.rows - 1) / p.cfg.rows), steps = (cap + p.cfg.keys - 1) / p.cfg.keys;
+  if (segs * steps >= (int64_t{1} << 30) || segs * num_seqs * steps >= (int64_t{1} << 30) ||
+      segs * num_seqs >= (int64_t{1} << 24))
+    return p;
   p.ok = true;
-  const int slots = (compute_units() * kWgPerCu + 7) / 8 * 8;
-  p.target = slots;
-  // Pieces: at most one per kMinSteps steps beside the last, and at most target + segments in all. A split segment has
-  // more than L >= total / target steps and at most steps / L + 1 pieces: at most 2 target records.
-  const int64_t cuts = (steps + kMinSteps - 1) / kMinSteps;
-  const int64_t pieces = segs * cuts < slots + segs ? segs * cuts : slots + segs;
-  p.grid = static_cast<int>((pieces < slots ? pieces : slots) + 7) / 8 * 8;
-  const int64_t recs = cuts > 1 ? (segs * cuts < 2 * slots ? segs * cuts : 2 * slots) : 0;
-  p.max_recs = static_cast<int>(recs);
-  p.desc_off = (recs * p.cfg.rec_floats * 4 + 255) / 256 * 256;
-  p.bytes = recs > 0 ? p.desc_off + recs * kDesc * 4 : 0;
+  p.segs_per_seq = static_cast<int>(segs);
+  p.min_share = (kMinShareKeys + p.cfg.keys - 1) / p.cfg.keys;
+  const int64_t most = (segs * num_seqs * steps + p.min_share - 1) / p.min_share, slots = compute_units() * p.cfg.occ;
+  p.grid = static_cast<int>((most < slots ? most : slots) + 7) / 8 * 8;
+  // A segment is split between two workers' shares, wherever it is longer than nothing: only a call whose segments
+  // are one step each has none.
+  if (steps > 1) {
+    p.start_off = (static_cast<int64_t>(p.grid) * 2 * p.cfg.rec_floats * 4 + 255) / 256 * 256;
+    p.bytes = p.start_off + (num_seqs + 1) * 4;
+  }
   return p;
 }
 
@@ -922,15 +1103,13 @@ extern "C" int mip_paged_tree(void* out, int64_t out_stride_tok, int64_t out_str
       if (!workspace || workspace_bytes < static_cast<size_t>(p.bytes) || (reinterpret_cast<uintptr_t>(workspace) & 255))
         return MIP_EINVAL;
       a.ws_rec = static_cast<float*>(workspace);
-      a.ws_desc = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + p.desc_off);
+      a.ws_start = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + p.start_off);
     }
-    a.rec_floats = p.cfg.rec_floats;
-    a.target = p.target;
-    a.min_steps = tree::kMinSteps;
-    a.max_recs = p.max_recs;
-    hipLaunchKernelGGL(p.cfg.fn, dim3(p.grid), dim3(p.cfg.threads), 0, s, a);
-    if (p.max_recs > 0)
-      hipLaunchKernelGGL(p.cfg.merge, dim3(p.max_recs, p.cfg.rows / 16), dim3(256), 0, s, a);
+    a.min_share = p.min_share;
+    hipLaunchKernelGGL(p.cfg.fn, dim3(p.grid), dim3(256), 0, s, a);
+    if (p.bytes > 0)
+      hipLaunchKernelGGL(p.cfg.merge, dim3(p.segs_per_seq * num_seqs, p.cfg.rows / 16), dim3(256), 0, s, a, p.segs_per_seq,
+                         p.cfg.keys);
     return status_from_hip(hipGetLastError());
   }
   const int64_t rows = static_cast<int64_t>(num_seqs) * max_q_len;
