@@ -51,6 +51,10 @@ typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint4 u4(const u32x4_t& x) { return __builtin_bit_cast(uint4, x); }
 
 constexpr int kMaxSeqs = 1024;  // sequences whose places fit in LDS
+#ifndef K_SLACK
+#define K_SLACK 4
+#endif
+constexpr int kSlack = K_SLACK;
 
 struct TreeArgs {
   char* out;
@@ -116,8 +120,7 @@ struct Shape {
   static constexpr int STAGE = 2 * TILE;           // shared: K | V of a step
   static constexpr int NLD = KT * CPR / T;         // shared: chunks a thread copies, each of K and V
   static constexpr int kRing = 2 * 64 * RB;        // private: a wavefront's two tiles of 32 K and 32 V rows
-  // The meeting of the WK wavefronts of a row goes through LDS one column block at a time.
-  static constexpr int kPark = NW * MT * kWave * 16;
+  static constexpr int kPark = NW * NC * MT * kWave * 16;  // every wavefront's sums, where the WK of a row meet
   static constexpr int kStages = kPrivate ? NW * kRing : 2 * STAGE;
   static constexpr int kLds = WK > 1 && kPark > kStages ? kPark : kStages;
   static constexpr int64_t kRec = 2 * R + static_cast<int64_t>(R) * D;  // floats of a record
@@ -161,7 +164,7 @@ __device__ __forceinline__ int keys_of(const TreeArgs& a, const Seq& q) {
   return q.ctx < cap - q.n ? q.ctx + q.n : cap;
 }
 
-// The query rows of a wavefront: row 16 c + lane % 16 of its NC column blocks, with its running softmax.
+// The query rows of a wavefront, NC column blocks of 16 (a lane's row in each: lane % 16), with their running softmax.
 template <int D, int NC>
 struct Rows {
   static constexpr int KC = D / 32, MT = D / 16;
@@ -172,10 +175,11 @@ struct Rows {
   f32x4_t l[NC];      // row sums by MFMA against a block of ones: every element holds the row's
   float m[NC];        // running maximum (log2 units)
 
-  __device__ __forceinline__ void load(const TreeArgs& a, const Piece& p, int first, int i16, int grp) {
+  // Blocks first, first + step, ..: row `block * 16 + i16` each.
+  __device__ __forceinline__ void load(const TreeArgs& a, const Piece& p, int first, int step, int i16, int grp) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const int r = first + c * 16 + i16;
+      const int r = (first + c * step) * 16 + i16;
       const int t = r / a.group, g = r - t * a.group;
       live[c] = t < p.q.n;
       tok[c] = live[c] ? t : 0;
@@ -376,11 +380,12 @@ __device__ __forceinline__ void careful_block(const TreeArgs& a, const Piece& p,
 }
 
 template <int DT, int D, int NC, int KT>
-__device__ __forceinline__ void careful_pass(const TreeArgs& a, const Piece& p, Rows<D, NC>& rows, int first, int wk, int lane) {
+__device__ __forceinline__ void careful_pass(const TreeArgs& a, const Piece& p, Rows<D, NC>& rows, int first, int step, int wk,
+                                             int lane) {
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     Rows<D, 1> one;
-    one.load(a, p, first + 16 * c, lane & 15, lane >> 4);
+    one.load(a, p, first + c * step, 0, lane & 15, lane >> 4);
     careful_block<DT, D, KT>(a, p, one, wk, lane);
     rows.m[c] = one.m[0];
     rows.l[c] = one.l[0];
@@ -543,10 +548,10 @@ __device__ __forceinline__ void private_pass(const TreeArgs& a, const Piece& p, 
 // A workgroup's keys of a piece, staged by all its threads for all its wavefronts: two LDS stages of a step, the
 // next step's rows in registers meanwhile. WR x WK wavefronts: WK take different 32 keys of a step. bf16 V is staged
 // as fp16, once for all rows.
-template <int DT, int D, int WR, int WK, int NC>
+template <int DT, int D, int WR, int WK, int NCK, int NC>
 __device__ __forceinline__ void shared_pass(const TreeArgs& a, const Piece& p, Rows<D, NC>& rows, char* smem, Shared& sh,
                                             int w, int lane) {
-  using P = Shape<D, WR, WK, NC>;
+  using P = Shape<D, WR, WK, NCK>;
   constexpr int KC = P::KC, MT = P::MT, RB = P::RB, CPR = P::CPR, NLD = P::NLD;
   const int tid = w * kWave + lane, wk = w % WK, i16 = lane & 15, grp = lane >> 4;
   const int32_t* table = a.bt + static_cast<int64_t>(p.s) * a.bt_stride;
@@ -644,6 +649,7 @@ __device__ __forceinline__ void put_block(const TreeArgs& a, const Piece& p, flo
   using Ops = MfmaOps<DT>;
   using S = typename Elem<DT>::S;
   const int i16 = lane & 15, grp = lane >> 4;
+  if (!__any(live)) return;
   if (rec) {
     f32x4_t* out = reinterpret_cast<f32x4_t*>(rec + 2 * R) + (cb * (D / 16) + mt0) * kWave + lane;
 #pragma unroll
@@ -666,32 +672,33 @@ __device__ __forceinline__ void put_block(const TreeArgs& a, const Piece& p, flo
   }
 }
 
-// One piece: rows of block p.rb against steps [p.step0, p.step1). rec: null where that is the whole segment.
-template <int DT, int D, int WR, int WK, int NC>
+// One piece: rows of block p.rb against steps [p.step0, p.step1). rec: null where that is the whole segment. NC: column
+// blocks of a wavefront here, at most the kernel's.
+template <int DT, int D, int WR, int WK, int NCK, int NC>
 __device__ __forceinline__ void run_piece(const TreeArgs& a, const Piece& p, float* rec, char* smem, Shared& sh,
-                                          float (*sh_ml)[4][16 * NC]) {
-  using P = Shape<D, WR, WK, NC>;
+                                          float (*sh_ml)[4][16 * NCK]) {
+  using P = Shape<D, WR, WK, NCK>;
   constexpr int MT = P::MT;
   const int lane = threadIdx.x & (kWave - 1);
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int wr = w / WK, wk = w % WK, i16 = lane & 15, grp = lane >> 4;
   Rows<D, NC> rows;
-  const int first = p.rb * P::R + wr * NC * 16;
-  rows.load(a, p, first, i16, grp);
+  const int first = p.rb * (P::R / 16) + wr;
+  rows.load(a, p, first, WR, i16, grp);
   if constexpr (P::kPrivate)
     private_pass<DT, D, NC>(a, p, rows, (lchar_t*)(smem + w * P::kRing), wk, lane);
   else
-    shared_pass<DT, D, WR, WK, NC>(a, p, rows, smem, sh, w, lane);
+    shared_pass<DT, D, WR, WK, NCK, NC>(a, p, rows, smem, sh, w, lane);
   // A wavefront whose accumulators hold inf or NaN does its part again.
-  if (!rows.finite()) careful_pass<DT, D, NC, P::KT>(a, p, rows, first, wk, lane);
+  if (!rows.finite()) careful_pass<DT, D, NC, P::KT>(a, p, rows, first, WR, wk, lane);
   if constexpr (WK == 1) {
 #pragma unroll
     for (int c = 0; c < NC; ++c)
-      put_block<DT, D, P::R, MT>(a, p, rec, wr * NC + c, 0, rows.live[c], rows.tok[c], rows.m[c], rows.l[c][0], rows.acc[c],
+      put_block<DT, D, P::R, MT>(a, p, rec, c * WR + wr, 0, rows.live[c], rows.tok[c], rows.m[c], rows.l[c][0], rows.acc[c],
                                  lane);
   } else {
     // The WK wavefronts of a row meet: each scales its sums to the common maximum, and each takes MT / WK of
-    // the dims of every column block, which go through LDS one block at a time.
+    // the dims of every column block.
     constexpr int PER = MT / WK;
     if (grp == 0) {
 #pragma unroll
@@ -702,31 +709,36 @@ __device__ __forceinline__ void run_piece(const TreeArgs& a, const Piece& p, flo
     }
     __syncthreads();  // also: every wavefront is done with its stage
     f32x4_t* park = reinterpret_cast<f32x4_t*>(smem);
+    float m[NC], l[NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      float m = -INFINITY, l = 0.0f;
+      m[c] = -INFINITY;
+      l[c] = 0.0f;
 #pragma unroll
-      for (int o = 0; o < WK; ++o) m = fmax2(m, sh_ml[0][wr * WK + o][c * 16 + i16]);
+      for (int o = 0; o < WK; ++o) m[c] = fmax2(m[c], sh_ml[0][wr * WK + o][c * 16 + i16]);
 #pragma unroll
       for (int o = 0; o < WK; ++o) {
         const float mo = sh_ml[0][wr * WK + o][c * 16 + i16];
         // A wavefront without keys has sums of 0 and a maximum of -inf (and so may all).
-        l += sh_ml[1][wr * WK + o][c * 16 + i16] * (mo == -INFINITY ? 0.0f : fast_exp2(mo - m));
+        l[c] += sh_ml[1][wr * WK + o][c * 16 + i16] * (mo == -INFINITY ? 0.0f : fast_exp2(mo - m[c]));
       }
-      const float f = rows.m[c] == -INFINITY ? 0.0f : fast_exp2(rows.m[c] - m);
+      const float f = rows.m[c] == -INFINITY ? 0.0f : fast_exp2(rows.m[c] - m[c]);
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) park[(w * MT + mt) * kWave + lane] = rows.acc[c][mt] * f;
-      __syncthreads();
+      for (int mt = 0; mt < MT; ++mt) park[((w * NC + c) * MT + mt) * kWave + lane] = rows.acc[c][mt] * f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
       f32x4_t sum[PER];
 #pragma unroll
       for (int x = 0; x < PER; ++x) {
-        sum[x] = park[((wr * WK) * MT + wk * PER + x) * kWave + lane];
+        sum[x] = park[((wr * WK * NC + c) * MT + wk * PER + x) * kWave + lane];
 #pragma unroll
-        for (int o = 1; o < WK; ++o) sum[x] += park[((wr * WK + o) * MT + wk * PER + x) * kWave + lane];
+        for (int o = 1; o < WK; ++o) sum[x] += park[(((wr * WK + o) * NC + c) * MT + wk * PER + x) * kWave + lane];
       }
-      put_block<DT, D, P::R, PER>(a, p, rec, wr * NC + c, wk * PER, rows.live[c], rows.tok[c], m, l, sum, lane);
-      __syncthreads();
+      put_block<DT, D, P::R, PER>(a, p, rec, c * WR + wr, wk * PER, rows.live[c], rows.tok[c], m[c], l[c], sum, lane);
     }
+    __syncthreads();  // the next piece fetches over the parked sums
   }
 }
 
@@ -768,6 +780,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
 
   // ---- equal shares: worker i takes steps [i * share, i * share + share). The workers of an XCD are neighbours, so
   // that row blocks of the same keys meet in its L2.
+  // A cut that falls close to a segment's end moves there, which spares a record and its combination.
   int share = (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
   share = share > a.min_share ? share : a.min_share;
   const int workers = (total + share - 1) / share, per_xcd = (workers + 7) / 8;
@@ -777,14 +790,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
     if (tid == 0) a.ws_start[S] = share;
   }
   if (static_cast<int>(blockIdx.x >> 3) >= per_xcd || worker >= workers) return;
-  int at = worker * share;
-  const int end = at + share < total ? at + share : total;
-  int lo = 0, hi = S - 1;  // the last sequence that starts at or before `at`
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (sh.start[mid] <= at) lo = mid; else hi = mid - 1;
-  }
-  for (int s = lo; at < end; ++s) {
+  const int slack = share / kSlack;
+  auto cut = [&](int at, int& s) {
+    if (at >= total) return total;
+    int lo = 0, hi = S - 1;  // the last sequence that starts at or before `at`
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (sh.start[mid] <= at) lo = mid; else hi = mid - 1;
+    }
+    s = __builtin_amdgcn_readfirstlane(lo);
+    const int nt = steps_of(seq_of(a, s)), into = (at - __builtin_amdgcn_readfirstlane(sh.start[s])) % nt;
+    return into < slack ? at - into : nt - into < slack ? at + nt - into : at;
+  };
+  int s = 0, dummy;
+  int at = cut(worker * share, s);
+  const int end = cut(worker * share + share, dummy);
+  for (; at < end; ++s) {
     Piece p;
     p.s = __builtin_amdgcn_readfirstlane(s);
     p.q = seq_of(a, p.s);
@@ -801,7 +822,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
       // A worker's first piece, if it begins inside its segment, has record 0, its last, if it ends inside, 1.
       if (p.step0 > 0 || p.step1 < nt)
         rec = a.ws_rec + (static_cast<int64_t>(worker) * 2 + (p.step0 > 0 ? 0 : 1)) * P::kRec;
-      run_piece<DT, D, WR, WK, NC>(a, p, rec, smem, sh, sh_ml);
+      // Column blocks that each wavefront has of the segment's, so that none is spent on rows that are none.
+      const int left = (p.q.n * a.group + 15) / 16 - p.rb * (P::R / 16);
+      const int nc = ((left < P::R / 16 ? left : P::R / 16) + WR - 1) / WR;
+      if (NC >= 4 && nc == 4) run_piece<DT, D, WR, WK, NC, NC < 4 ? NC : 4>(a, p, rec, smem, sh, sh_ml);
+      else if (NC >= 3 && nc == 3) run_piece<DT, D, WR, WK, NC, NC < 3 ? NC : 3>(a, p, rec, smem, sh, sh_ml);
+      else if (NC >= 2 && nc == 2) run_piece<DT, D, WR, WK, NC, NC < 2 ? NC : 2>(a, p, rec, smem, sh, sh_ml);
+      else run_piece<DT, D, WR, WK, NC, 1>(a, p, rec, smem, sh, sh_ml);
       at = seg0 + p.step1;
     }
   }
@@ -819,8 +846,11 @@ __global__ __launch_bounds__(256) void paged_tree_merge(TreeArgs a, int segs_per
   const int first = a.ws_start[s], share = a.ws_start[a.num_seqs];
   const int nt = (keys_of(a, p.q) + keys_per_step - 1) / keys_per_step, segs = segments_of(a, p.q, R), nrb = segs / a.hkv;
   if (seg >= segs) return;
-  const int begin = first + seg * nt, w0 = begin / share, w1 = (begin + nt - 1) / share;
-  if (w0 == w1) return;
+  // The cuts inside the segment: the multiples of `share` that did not move to one of its ends. Worker w0 has the
+  // first piece, w0 + 1 .. w1 have the others.
+  const int begin = first + seg * nt, slack = share / kSlack, near = slack > 1 ? slack : 1;
+  const int w0 = (begin + near - 1) / share, w1 = (begin + nt - near) / share;
+  if (w0 >= w1) return;
   p.kvh = seg / nrb;
   p.rb = seg - p.kvh * nrb;
   const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave, i16 = lane & 15;
@@ -883,36 +913,51 @@ __global__ __launch_bounds__(256) void paged_tree_row_kernel(TreeArgs a, int hq)
     acc[e] = 0.0f;
   }
   float m = -INFINITY, l = 0.0f;
-  auto values = [&](const char* pool, int64_t at, float (&v)[N]) {
-    const uint4 u = *reinterpret_cast<const uint4*>(pool + at);
-    S raw[N];
-    __builtin_memcpy(raw, &u, 16);
+  // A step: U keys for every row of lanes, their block ids read one step ahead and all of their K and V
+  // requested before any is used.
+  constexpr int U = RPP >= 16 ? 1 : RPP >= 8 ? 2 : 4, STEP = 4 * RPP * U;
+  int ids[U];
+  bool in[U];
+  auto lookup = [&](int base) __attribute__((always_inline)) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = widen<DT>(raw[e]);
+    for (int u = 0; u < U; ++u) {
+      const int key = base + (u * 4 + w) * RPP + row, e0 = key - p.ctx;
+      in[u] = key < keys;
+      ids[u] = in[u] ? table[key >> a.log2_bs] : -1;
+      if (in[u] && e0 >= 0) in[u] = (e0 >> 6) < a.mask_words && ((mask[e0 >> 6] >> (e0 & 63)) & 1u);
+    }
   };
-  for (int base = 0; base < keys; base += 4 * RPP) {
-    const int key = base + w * RPP + row, e0 = key - p.ctx;
-    bool seen = key < keys;
-    if (seen && e0 >= 0) seen = (e0 >> 6) < a.mask_words && ((mask[e0 >> 6] >> (e0 & 63)) & 1u);
-    const int blk = seen ? table[key >> a.log2_bs] : -1;
-    seen = blk >= 0 && blk < a.ncb;
-    const int64_t at = (((static_cast<int64_t>(seen ? blk : 0) * a.hkv + kvh) * a.bs + (key & (a.bs - 1))) * D + c * N) * ES;
-    float kf[N];
-    values(a.k, at, kf);
-    float dot = 0.0f;
+  lookup(0);
+  for (int base = 0; base < keys; base += STEP) {
+    u32x4_t kw[U], vw[U];
+    bool seen[U];
 #pragma unroll
-    for (int e = 0; e < N; ++e) dot = fmaf(qf[e], kf[e], dot);
+    for (int u = 0; u < U; ++u) {
+      const int key = base + (u * 4 + w) * RPP + row;
+      const bool ok = ids[u] >= 0 && ids[u] < a.ncb;
+      seen[u] = ok && in[u];
+      const int64_t at =
+          (((static_cast<int64_t>(ok ? ids[u] : 0) * a.hkv + kvh) * a.bs + (key & (a.bs - 1))) * D + c * N) * ES;
+      kw[u] = *reinterpret_cast<const u32x4_t*>(a.k + at);
+      vw[u] = *reinterpret_cast<const u32x4_t*>(a.v + at);
+    }
+    if (base + STEP < keys) lookup(base + STEP);
 #pragma unroll
-    for (int o = 1; o < LPR; o <<= 1) dot += __shfl_xor(dot, o);
-    if (seen && dot != -INFINITY) {
-      float vf[N];
-      values(a.v, at, vf);
-      const float sc = dot * a.scale_log2;
-      const float mn = fmax2(m, sc);
+    for (int u = 0; u < U; ++u) {
+      S kr[N], vr[N];
+      __builtin_memcpy(kr, &kw[u], 16);
+      __builtin_memcpy(vr, &vw[u], 16);
+      float dot = 0.0f;
+#pragma unroll
+      for (int e = 0; e < N; ++e) dot = fmaf(qf[e], widen<DT>(kr[e]), dot);
+#pragma unroll
+      for (int o = 1; o < LPR; o <<= 1) dot += __shfl_xor(dot, o);
+      if (!seen[u] || dot == -INFINITY) continue;
+      const float sc = dot * a.scale_log2, mn = fmax2(m, sc);
       const float alpha = fast_exp2(m - mn), pk = fast_exp2(sc - mn);  // m = -inf before any key: alpha 0
       l = l * alpha + pk;
 #pragma unroll
-      for (int e = 0; e < N; ++e) acc[e] = fmaf(pk, vf[e], acc[e] * alpha);
+      for (int e = 0; e < N; ++e) acc[e] = fmaf(pk, widen<DT>(vr[e]), acc[e] * alpha);
       m = mn;
     }
   }
@@ -972,7 +1017,7 @@ Config pick(int d, int64_t rows) {
   return config_of<DT, 128, 4, 1, 2, 2>();
 }
 
-constexpr int kMinShareKeys = 256;  // fewest keys a worker takes
+constexpr int kMinShareKeys = 64;  // fewest keys a worker takes
 
 int compute_units() {
   int dev = 0, cus = 0;

@@ -18,8 +18,10 @@ namespace mip {
 namespace {
 
 template <int CHUNK> struct MoveT;
-template <> struct MoveT<16> { using T = uint4; };
-template <> struct MoveT<8>  { using T = uint2; };
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+template <> struct MoveT<16> { using T = u32x4_t; };  // (an array of uint4 would stay in scratch memory)
+template <> struct MoveT<8>  { using T = u32x2_t; };
 template <> struct MoveT<4>  { using T = uint32_t; };
 template <> struct MoveT<2>  { using T = uint16_t; };
 
