@@ -51,10 +51,6 @@ typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint4 u4(const u32x4_t& x) { return __builtin_bit_cast(uint4, x); }
 
 constexpr int kMaxSeqs = 1024;  // sequences whose places fit in LDS
-#ifndef K_SLACK
-#define K_SLACK 4
-#endif
-constexpr int kSlack = K_SLACK;
 
 struct TreeArgs {
   char* out;
@@ -72,12 +68,19 @@ struct TreeArgs {
   int64_t mask_st;         // words
   int mask_words;
   int hkv, group, bs, log2_bs, max_blocks;
+  uint32_t group_inv;      // ceil(2^32 / group): r / group = high word of r * group_inv while r * group < 2^32
   int num_seqs, max_q_len;
   float scale_log2;
   int min_share;           // fewest steps a worker takes
+  int slack;               // a cut this many steps or closer to a segment's end moves there
   float* ws_rec;           // two records a worker: m[R] | l[R] | accumulators
   int32_t* ws_start;       // first step of every sequence, then the steps of a share (null: no segment is split)
 };
+
+// Steps from a segment's end within which a cut moves there, which spares a record and its combination.
+__device__ __forceinline__ int slack_of(const TreeArgs& a, int share) {
+  return share / 8 > a.slack ? share / 8 : a.slack;
+}
 
 __device__ __forceinline__ float fmax2(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 __device__ __forceinline__ float fmax3(float a, float b, float c) { return fmax2(fmax2(a, b), c); }
@@ -144,18 +147,26 @@ struct Piece {
 struct Shared {
   int scan[4];
   int start[kMaxSeqs];  // first step of every sequence's segments
+  int cu[kMaxSeqs + 1], ctx[kMaxSeqs];
   uint32_t ok[2];       // byte w: every key that wavefront w copied exists and lies in a block of the pool
 };
 
-__device__ __forceinline__ Seq seq_of(const TreeArgs& a, int s) {
+// Node of query row r (group 1 has no 32-bit reciprocal).
+__device__ __forceinline__ int node_of(const TreeArgs& a, int r) {
+  return a.group_inv ? static_cast<int>(__umulhi(static_cast<uint32_t>(r), a.group_inv)) : r;
+}
+
+__device__ __forceinline__ Seq seq_of(const TreeArgs& a, int q0, int q1, int ctx) {
   Seq q;
-  q.q0 = a.cu_q[s];
-  q.n = a.cu_q[s + 1] - q.q0;
+  q.q0 = q0;
+  q.n = q1 - q0;
   q.n = q.n < a.max_q_len ? q.n : a.max_q_len;
   q.n = q.n > 0 ? q.n : 0;
-  q.ctx = a.ctx_start[s];
-  q.ctx = q.ctx > 0 ? q.ctx : 0;
+  q.ctx = ctx > 0 ? ctx : 0;
   return q;
+}
+__device__ __forceinline__ Seq seq_of(const TreeArgs& a, int s) {
+  return seq_of(a, a.cu_q[s], a.cu_q[s + 1], a.ctx_start[s]);
 }
 
 // Keys of a sequence; those past the table are never read.
@@ -180,7 +191,7 @@ struct Rows {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int r = (first + c * step) * 16 + i16;
-      const int t = r / a.group, g = r - t * a.group;
+      const int t = node_of(a, r), g = r - t * a.group;
       live[c] = t < p.q.n;
       tok[c] = live[c] ? t : 0;
       const char* row = a.q + ((static_cast<int64_t>(p.q.q0) + tok[c]) * a.q_st +
@@ -661,7 +672,7 @@ __device__ __forceinline__ void put_block(const TreeArgs& a, const Piece& p, flo
     return;
   }
   if (!live) return;
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // 0: no key seen, sums of 0
+  const float inv = l == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(l);  // to 2^-23; 0: no key seen, sums of 0
   const int r = p.rb * R + cb * 16 + i16;
   S* row = reinterpret_cast<S*>(a.out) + (static_cast<int64_t>(p.q.q0) + tok) * a.out_st +
            static_cast<int64_t>(p.kvh * a.group + r - tok * a.group) * a.out_sh;
@@ -762,7 +773,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
     const int s = s0 + tid;
     int n = 0;
     if (s < S) {
-      const Seq q = seq_of(a, s);
+      const int q0 = a.cu_q[s], q1 = a.cu_q[s + 1], ctx = a.ctx_start[s];
+      const Seq q = seq_of(a, q0, q1, ctx);
+      sh.cu[s] = q0;
+      if (s == S - 1) sh.cu[S] = q1;
+      sh.ctx[s] = ctx;
       n = segments_of(a, q, P::R) * steps_of(q);
     }
     const int incl = decode::wave_inclusive_scan(n, lane);
@@ -780,7 +795,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
 
   // ---- equal shares: worker i takes steps [i * share, i * share + share). The workers of an XCD are neighbours, so
   // that row blocks of the same keys meet in its L2.
-  // A cut that falls close to a segment's end moves there, which spares a record and its combination.
   int share = (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
   share = share > a.min_share ? share : a.min_share;
   const int workers = (total + share - 1) / share, per_xcd = (workers + 7) / 8;
@@ -790,7 +804,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
     if (tid == 0) a.ws_start[S] = share;
   }
   if (static_cast<int>(blockIdx.x >> 3) >= per_xcd || worker >= workers) return;
-  const int slack = share / kSlack;
+  const int slack = slack_of(a, share);
+  auto known = [&](int s) {
+    Seq q = seq_of(a, sh.cu[s], sh.cu[s + 1], sh.ctx[s]);
+    return Seq{__builtin_amdgcn_readfirstlane(q.q0), __builtin_amdgcn_readfirstlane(q.n),
+               __builtin_amdgcn_readfirstlane(q.ctx)};
+  };
   auto cut = [&](int at, int& s) {
     if (at >= total) return total;
     int lo = 0, hi = S - 1;  // the last sequence that starts at or before `at`
@@ -799,7 +818,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
       if (sh.start[mid] <= at) lo = mid; else hi = mid - 1;
     }
     s = __builtin_amdgcn_readfirstlane(lo);
-    const int nt = steps_of(seq_of(a, s)), into = (at - __builtin_amdgcn_readfirstlane(sh.start[s])) % nt;
+    const int nt = steps_of(known(s)), into = (at - __builtin_amdgcn_readfirstlane(sh.start[s])) % nt;
     return into < slack ? at - into : nt - into < slack ? at + nt - into : at;
   };
   int s = 0, dummy;
@@ -808,9 +827,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
   for (; at < end; ++s) {
     Piece p;
     p.s = __builtin_amdgcn_readfirstlane(s);
-    p.q = seq_of(a, p.s);
+    p.q = known(p.s);
     p.last = keys_of(a, p.q) - 1;
-    const int nt = steps_of(p.q), segs = segments_of(a, p.q, P::R), nrb = segs / a.hkv;
+    const int nt = steps_of(p.q), nrb = (p.q.n * a.group + P::R - 1) / P::R, segs = nrb * a.hkv;
     const int first = __builtin_amdgcn_readfirstlane(sh.start[s]);
     while (at < end && at < first + segs * nt) {
       const int seg = (at - first) / nt, seg0 = first + seg * nt;
@@ -834,49 +853,75 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
   }
 }
 
-// Combine the pieces of a split segment. Workgroup (x, cb): column block cb of segment x = (sequence, (kv head, row block));
-// each wavefront a quarter of the dims.
-template <int DT, int D, int R>
+// Combine the pieces of a split segment. Workgroup (x, cb, z): column block cb of segment x = (sequence, (kv head, row
+// block)). BY_PIECE: two dim tiles (z) of the block, each wavefront a quarter of the pieces (few segments, cut into many
+// pieces each: more workgroups and shorter chains); else all its dims, each wavefront a quarter of them.
+template <int DT, int D, int R, bool BY_PIECE>
 __global__ __launch_bounds__(256) void paged_tree_merge(TreeArgs a, int segs_per_seq, int keys_per_step) {
-  constexpr int MT = D / 16, PER = MT / 4;
+  constexpr int MT = D / 16, PER = BY_PIECE ? 2 : MT / 4;
   const int s = blockIdx.x / segs_per_seq, seg = blockIdx.x - s * segs_per_seq, cb = blockIdx.y;
   Piece p;
   p.s = s;
   p.q = seq_of(a, s);
   const int first = a.ws_start[s], share = a.ws_start[a.num_seqs];
-  const int nt = (keys_of(a, p.q) + keys_per_step - 1) / keys_per_step, segs = segments_of(a, p.q, R), nrb = segs / a.hkv;
+  const int nt = (keys_of(a, p.q) + keys_per_step - 1) / keys_per_step;
+  const int nrb = (p.q.n * a.group + R - 1) / R, segs = nrb * a.hkv;
   if (seg >= segs) return;
   // The cuts inside the segment: the multiples of `share` that did not move to one of its ends. Worker w0 has the
   // first piece, w0 + 1 .. w1 have the others.
-  const int begin = first + seg * nt, slack = share / kSlack, near = slack > 1 ? slack : 1;
+  const int begin = first + seg * nt, near = slack_of(a, share);
   const int w0 = (begin + near - 1) / share, w1 = (begin + nt - near) / share;
   if (w0 >= w1) return;
   p.kvh = seg / nrb;
   p.rb = seg - p.kvh * nrb;
-  const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave, i16 = lane & 15;
   if (p.rb * R + cb * 16 >= p.q.n * a.group) return;
+  const int lane = threadIdx.x & (kWave - 1), i16 = lane & 15, w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int mt0 = BY_PIECE ? 2 * blockIdx.z : w * PER;
   constexpr int64_t kRec = 2 * R + static_cast<int64_t>(R) * D;
   // The segment's first piece ends inside it (record 1 of its worker); the others begin inside it (record 0).
   auto record = [&](int x) { return a.ws_rec + (static_cast<int64_t>(x) * 2 + (x == w0 ? 1 : 0)) * kRec; };
-  float m = -INFINITY;
-#pragma unroll 4
-  for (int x = w0; x <= w1; ++x) m = fmax2(m, record(x)[cb * 16 + i16]);
-  float l = 0.0f;
+  const int from = BY_PIECE ? w0 + (w1 - w0 + 1) * w / 4 : w0, to = BY_PIECE ? w0 + (w1 - w0 + 1) * (w + 1) / 4 : w1 + 1;
+  float m = -INFINITY, l = 0.0f;
+#pragma unroll 8
+  for (int x = from; x < to; ++x) m = fmax2(m, record(x)[cb * 16 + i16]);
   f32x4_t acc[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) acc[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-  for (int x = w0; x <= w1; ++x) {
+#pragma unroll 8
+  for (int x = from; x < to; ++x) {
     const float* rec = record(x);
     const float mp = rec[cb * 16 + i16];
     const float f = mp == -INFINITY ? 0.0f : fast_exp2(mp - m);
     l += f * rec[R + cb * 16 + i16];
-    const f32x4_t* racc = reinterpret_cast<const f32x4_t*>(rec + 2 * R) + (cb * MT + w * PER) * kWave + lane;
+    const f32x4_t* racc = reinterpret_cast<const f32x4_t*>(rec + 2 * R) + (cb * MT + mt0) * kWave + lane;
 #pragma unroll
     for (int i = 0; i < PER; ++i) acc[i] += racc[i * kWave] * f;
   }
-  const int r = p.rb * R + cb * 16 + i16, tok = r / a.group;
-  put_block<DT, D, R, PER>(a, p, nullptr, cb, w * PER, tok < p.q.n, tok, m, l, acc, lane);
+  if constexpr (BY_PIECE) {
+    __shared__ float s_ml[2][4][16];
+    __shared__ f32x4_t s_acc[4][PER][kWave];
+    if (lane < 16) {
+      s_ml[0][w][i16] = m;
+      s_ml[1][w][i16] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) s_acc[w][i][lane] = acc[i];
+    __syncthreads();
+    if (w > 0) return;
+    m = fmax2(fmax2(s_ml[0][0][i16], s_ml[0][1][i16]), fmax2(s_ml[0][2][i16], s_ml[0][3][i16]));
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) acc[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int o = 0; o < 4; ++o) {
+      const float mo = s_ml[0][o][i16], f = mo == -INFINITY ? 0.0f : fast_exp2(mo - m);
+      l += f * s_ml[1][o][i16];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) acc[i] += s_acc[o][i][lane] * f;
+    }
+  }
+  const int r = p.rb * R + cb * 16 + i16, tok = node_of(a, r);
+  put_block<DT, D, R, PER>(a, p, nullptr, cb, mt0, tok < p.q.n, tok, m, l, acc, lane);
 }
 
 // ------------------------------------------------------------------ one query row at a time
@@ -990,7 +1035,7 @@ using MergeFn = void (*)(TreeArgs, int, int);
 
 struct Config {
   KernelFn fn = nullptr;
-  MergeFn merge = nullptr;
+  MergeFn merge = nullptr, merge_by_piece = nullptr;
   int rows = 0, keys = 0, occ = 0;  // R, KT, workgroups per CU
   int64_t rec_floats = 0;
 };
@@ -998,7 +1043,8 @@ struct Config {
 template <int DT, int D, int WR, int WK, int NC, int OCC>
 Config config_of() {
   using P = Shape<D, WR, WK, NC>;
-  return {paged_tree_kernel<DT, D, WR, WK, NC, OCC>, paged_tree_merge<DT, D, P::R>, P::R, P::KT, OCC, P::kRec};
+  return {paged_tree_kernel<DT, D, WR, WK, NC, OCC>, paged_tree_merge<DT, D, P::R, false>,
+          paged_tree_merge<DT, D, P::R, true>, P::R, P::KT, OCC, P::kRec};
 }
 
 // The workgroup's shape by the most rows a sequence can have.
@@ -1017,6 +1063,10 @@ Config pick(int d, int64_t rows) {
   return config_of<DT, 128, 4, 1, 2, 2>();
 }
 
+#ifndef K_BYP
+#define K_BYP 512
+#endif
+constexpr unsigned kMergeByPiece = K_BYP;
 constexpr int kMinShareKeys = 64;  // fewest keys a worker takes
 
 int compute_units() {
@@ -1029,7 +1079,7 @@ int compute_units() {
 struct Plan {
   Config cfg;
   bool ok = false;      // the matrix-core kernel takes this shape
-  int grid = 0, segs_per_seq = 0, min_share = 0;
+  int grid = 0, segs_per_seq = 0, min_share = 0, slack = 1;
   int64_t start_off = 0, bytes = 0;  // bytes 0: no segment can be split
 };
 
@@ -1040,7 +1090,7 @@ Plan plan_of(int num_seqs, int max_q_len, int hq, int hkv, int d, int bs, int ma
   if ((dtype != MIP_F16 && dtype != MIP_BF16) || (d != 64 && d != 128) || num_seqs > kMaxSeqs) return p;
   p.cfg = dtype == MIP_F16 ? pick<MIP_F16>(d, rows) : pick<MIP_BF16>(d, rows);
   const int64_t segs = hkv * ((rows + p.cfg.rows - 1) / p.cfg.rows), steps = (cap + p.cfg.keys - 1) / p.cfg.keys;
-  if (segs * steps >= (int64_t{1} << 30) || segs * num_seqs * steps >= (int64_t{1} << 30) ||
+  if ((rows + 256) * group >= (int64_t{1} << 31) || segs * steps >= (int64_t{1} << 30) || segs * num_seqs * steps >= (int64_t{1} << 30) ||
       segs * num_seqs >= (int64_t{1} << 24))
     return p;
   p.ok = true;
@@ -1048,13 +1098,27 @@ Plan plan_of(int num_seqs, int max_q_len, int hq, int hkv, int d, int bs, int ma
   p.min_share = (kMinShareKeys + p.cfg.keys - 1) / p.cfg.keys;
   const int64_t most = (segs * num_seqs * steps + p.min_share - 1) / p.min_share, slots = compute_units() * p.cfg.occ;
   p.grid = static_cast<int>((most < slots ? most : slots) + 7) / 8 * 8;
-  // A segment is split between two workers' shares, wherever it is longer than nothing: only a call whose segments
-  // are one step each has none.
-  if (steps > 1) {
+  // Short segments are left whole where there are enough of them for the chip (graph replay, us, cut / whole;
+  // sequences x nodes over 256-512 keys, 14q/2kv d64: 64 x 2 11.0/10.6, 64 x 8 17.3/15.4, 256 x 4 23.5/18.6, 256 x 64
+  // 82.1/70.6; 28q/4kv d128 over 512-1024: 16 x 8 24.6/22.2, 64 x 8 46.4/43.7) and cut where there are few (64 nodes
+  // over 250 keys 13.6/18.8; 4 x 64 over 512 16.2/23.9; d128 4 x 8 15.7/17.5, 64 x 16 41.3/47.9).
+  const int64_t all = segs * num_seqs;
+  if (p.cfg.keys >= 128 ? 4 * all >= p.grid : all >= 2 * p.grid) p.slack = (d == 64 ? 384 : 256) / p.cfg.keys;
+  if (steps >= 2 * p.slack) {  // else no cut stays inside a segment
     p.start_off = (static_cast<int64_t>(p.grid) * 2 * p.cfg.rec_floats * 4 + 255) / 256 * 256;
     p.bytes = p.start_off + (num_seqs + 1) * 4;
   }
   return p;
+}
+
+// Where the row kernel beats the matrix-core kernel in 16 bits: a workgroup for each (node, head) reads the keys
+// again, so it wins while they are few and so are the rows (graph replay, us, row / matrix cores; sequences x nodes,
+// 14q/2kv d64: 1 x 5 over 60 keys 4.4/7.2, 500 8.9/10.3, 1000 14.6/11.0; 1 x 64 120 6.9/13.0, 500 13.5/14.4;
+// 32 x 5 16 6.4/8.0, 120 8.8/8.1; 8 x 24 60 9.1/13.9, 250 16.6/15.7; 28q/4kv d128: 1 x 5 250 8.6/12.5, 500 14.6/12.8;
+// 8 x 5 120 9.0/9.8, 250 14.4/13.6; 32 x 5 16 13.7/9.9).
+bool row_kernel_pays(int num_seqs, int max_q_len, int hq, int d, int64_t cap) {
+  const int64_t rows = static_cast<int64_t>(num_seqs) * max_q_len * hq;
+  return cap * d <= 49152 && rows * cap * d <= (int64_t{1} << 24);
 }
 
 template <int DT>
@@ -1130,6 +1194,7 @@ extern "C" int mip_paged_tree(void* out, int64_t out_stride_tok, int64_t out_str
   a.mask_words = mask_words;
   a.hkv = num_kv_heads;
   a.group = num_heads / num_kv_heads;
+  a.group_inv = a.group > 1 ? static_cast<uint32_t>(((uint64_t{1} << 32) + a.group - 1) / a.group) : 0;
   a.bs = block_size;
   a.log2_bs = ilog2_exact(block_size);
   a.max_blocks = max_blocks_per_seq;
@@ -1143,7 +1208,7 @@ extern "C" int mip_paged_tree(void* out, int64_t out_stride_tok, int64_t out_str
                            ? tree::Plan{}
                            : tree::plan_of(num_seqs, max_q_len, num_heads, num_kv_heads, head_dim, block_size,
                                            max_blocks_per_seq, dtype);
-  if (p.ok) {
+  if (p.ok && !tree::row_kernel_pays(num_seqs, max_q_len, num_heads, head_dim, cap)) {
     if (p.bytes > 0) {
       if (!workspace || workspace_bytes < static_cast<size_t>(p.bytes) || (reinterpret_cast<uintptr_t>(workspace) & 255))
         return MIP_EINVAL;
@@ -1151,10 +1216,17 @@ extern "C" int mip_paged_tree(void* out, int64_t out_stride_tok, int64_t out_str
       a.ws_start = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + p.start_off);
     }
     a.min_share = p.min_share;
+    a.slack = p.slack;
     hipLaunchKernelGGL(p.cfg.fn, dim3(p.grid), dim3(256), 0, s, a);
-    if (p.bytes > 0)
-      hipLaunchKernelGGL(p.cfg.merge, dim3(p.segs_per_seq * num_seqs, p.cfg.rows / 16), dim3(256), 0, s, a, p.segs_per_seq,
-                         p.cfg.keys);
+    if (p.bytes > 0) {
+      const unsigned segs = static_cast<unsigned>(p.segs_per_seq * num_seqs), blocks = p.cfg.rows / 16;
+      // Few workgroups by column block: each segment has many pieces.
+      if (segs * blocks <= tree::kMergeByPiece)
+        hipLaunchKernelGGL(p.cfg.merge_by_piece, dim3(segs, blocks, head_dim / 32), dim3(256), 0, s, a, p.segs_per_seq,
+                           p.cfg.keys);
+      else
+        hipLaunchKernelGGL(p.cfg.merge, dim3(segs, blocks), dim3(256), 0, s, a, p.segs_per_seq, p.cfg.keys);
+    }
     return status_from_hip(hipGetLastError());
   }
   const int64_t rows = static_cast<int64_t>(num_seqs) * max_q_len;
