@@ -97,8 +97,9 @@ __device__ __forceinline__ void f32_load_v(float (&v)[4][D / 16], const DecodeAr
   }
 }
 
-template <int D>
-__global__ __launch_bounds__(kNW * kWave) void paged_attn_f32(DecodeArgs a) {
+// TREE: packed nodes of drafted trees; a row's own keys come from its mask instead of its position.
+template <int D, bool TREE>
+__device__ __forceinline__ void attn_f32(const DecodeArgs& a, const TreeMask& tm) {
   constexpr int T = D / 16;  // dim tiles
   __shared__ float sh_acc[kNW][kRows][D + 4];  // + 4: the 16 rows of a store spread over the banks
   __shared__ float sh_m[kNW][kRows], sh_l[kNW][kRows];
@@ -109,11 +110,16 @@ __global__ __launch_bounds__(kNW * kWave) void paged_attn_f32(DecodeArgs a) {
   // The workgroup's rows: row r is query row q0 + r / group of q, head kvh * group + r % group,
   // from row r0 on; it sees keys below first + r / group (decode: one token, the whole context).
   int part = 0, q0, r0, rows, trow, first;
-  if (a.cu_q) {
+  if (TREE || a.cu_q) {
     const int tiles = (a.max_q_len * a.group + kRows - 1) / kRows;
     const int s = blockIdx.x / tiles;
     q0 = a.cu_q[s];
-    rows = (a.cu_q[s + 1] - q0) * a.group;
+    if constexpr (TREE) {
+      rows = min(a.cu_q[s + 1] - q0, a.max_q_len) * a.group;
+      part = blockIdx.z;
+    } else {
+      rows = (a.cu_q[s + 1] - q0) * a.group;
+    }
     r0 = (blockIdx.x - s * tiles) * kRows;
     if (r0 >= rows) return;
     trow = s;
@@ -127,11 +133,13 @@ __global__ __launch_bounds__(kNW * kWave) void paged_attn_f32(DecodeArgs a) {
   }
   const int cap = a.max_blocks * a.bs;
   const int last_row = r0 + kRows < rows ? r0 + kRows - 1 : rows - 1;
-  const int ctx = min(first + last_row / a.group, cap);  // keys of the row that sees most
-  const int np_b = !a.cu_q && ctx > 0 ? (ctx + a.part_tokens - 1) / a.part_tokens : 1;
+  const int cached = max(first - 1, 0);  // TREE: keys that every row sees
+  const int ctx = TREE ? (cached < cap - rows / a.group ? cached + rows / a.group : cap)  // the sequence's keys
+                       : min(first + last_row / a.group, cap);  // keys of the row that sees most
+  const int np_b = (TREE || !a.cu_q) && ctx > 0 ? (ctx + a.part_tokens - 1) / a.part_tokens : 1;
   if (part >= np_b) return;
   const int t0 = part * a.part_tokens;
-  const int t1 = a.cu_q ? ctx : min(t0 + a.part_tokens, ctx);
+  const int t1 = !TREE && a.cu_q ? ctx : min(t0 + a.part_tokens, ctx);
 
   const int row = min(r0 + c, last_row);  // rows past the end shadow the last one
   const int row_tok = row / a.group;
@@ -142,7 +150,8 @@ __global__ __launch_bounds__(kNW * kWave) void paged_attn_f32(DecodeArgs a) {
 #pragma unroll
   for (int i = 0; i < D / 4; ++i) qf[i] = qp[i];
   // Keys below this are seen by every row.
-  const int all_see = min(first + r0 / a.group, cap);
+  const int all_see = TREE ? cached : min(first + r0 / a.group, cap);
+  const uint64_t* mask_row = TREE ? tm.mask + (static_cast<int64_t>(q0) + row_tok) * tm.stride : nullptr;
 
   float m = kNoScore, l = 0.f;
   f32x4_t acc[T];
@@ -182,10 +191,13 @@ __global__ __launch_bounds__(kNW * kWave) void paged_attn_f32(DecodeArgs a) {
     }
     f32_load_k<D>(kf, a, at, g);
     bool need = false;
+    // TREE: bit k: this lane's row sees key base + k.
+    const uint32_t sees = TREE ? valid & (base + 16 > cached ? tree_window(mask_row, tm.words, base - cached) : 0xffffu) : 0u;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int key = 4 * g + i;
-      s[i] = ((valid >> key) & 1u) && base + key < lim ? s[i] * a.scale_log2 : -INFINITY;
+      const bool seen = TREE ? (sees >> key) & 1u : ((valid >> key) & 1u) && base + key < lim;
+      s[i] = seen ? s[i] * a.scale_log2 : -INFINITY;
       need |= s[i] > m + kRescaleLog2;
     }
     if (__any(need)) {
@@ -234,7 +246,7 @@ __global__ __launch_bounds__(kNW * kWave) void paged_attn_f32(DecodeArgs a) {
             const bool wild = !(fabsf(x) < INFINITY);
             const float pk = key % 4 == 0 ? p[0] : key % 4 == 1 ? p[1] : key % 4 == 2 ? p[2] : p[3];
             const float pr = __shfl(pk, (key / 4) * 16 + c);
-            if (wild && base + key < lim) acc[t][i] += pr * x;
+            if (wild && (TREE ? (sees >> key) & 1u : base + key < lim)) acc[t][i] += pr * x;
           }
         }
       }
@@ -279,9 +291,10 @@ __global__ __launch_bounds__(kNW * kWave) void paged_attn_f32(DecodeArgs a) {
     }
     const int tok = (r0 + r) / a.group, head = kvh * a.group + (r0 + r) - tok * a.group;
     if (np_b == 1) {
-      out[(q0 + tok) * a.out_sb + head * a.out_sh + d] = Ls > 0.f ? A / Ls : 0.f;
+      // (A NaN among a tree row's scores has to stay one.)
+      out[(q0 + tok) * a.out_sb + head * a.out_sh + d] = (TREE ? Ls != 0.f : Ls > 0.f) ? A / Ls : 0.f;
     } else {
-      const int64_t slot = (static_cast<int64_t>(q0) * a.hq + head) * a.nparts + part;
+      const int64_t slot = (static_cast<int64_t>(TREE ? q0 + tok : q0) * a.hq + head) * a.nparts + part;
       a.ws_acc[slot * D + d] = A;
       if (d == 0) {
         a.ws_ml[slot * 2] = mx;
@@ -289,6 +302,16 @@ __global__ __launch_bounds__(kNW * kWave) void paged_attn_f32(DecodeArgs a) {
       }
     }
   }
+}
+
+template <int D>
+__global__ __launch_bounds__(kNW * kWave) void paged_attn_f32(DecodeArgs a) {
+  attn_f32<D, false>(a, TreeMask{});
+}
+
+template <int D>
+__global__ __launch_bounds__(kNW * kWave) void paged_tree_f32(DecodeArgs a, TreeMask t) {
+  attn_f32<D, true>(a, t);
 }
 
 }  // namespace
@@ -300,6 +323,16 @@ int f32_prefill_launch(const DecodeArgs& a, int num_seqs, int d, hipStream_t str
   const int64_t tiles = (static_cast<int64_t>(a.max_q_len) * a.group + kRows - 1) / kRows;
   hipLaunchKernelGGL(f32_decode_kernel(d), dim3(static_cast<unsigned>(tiles * num_seqs), a.hkv), dim3(kNW * kWave), 0,
                      stream, a);
+  return status_from_hip(hipGetLastError());
+}
+
+int f32_tree_launch(const DecodeArgs& a, const TreeMask& t, int num_seqs, int d, hipStream_t stream) {
+  const int64_t tiles = (static_cast<int64_t>(a.max_q_len) * a.group + kRows - 1) / kRows;
+  const dim3 grid(static_cast<unsigned>(tiles * num_seqs), a.hkv, a.nparts), block(kNW * kWave);
+  if (d == 64)
+    hipLaunchKernelGGL(paged_tree_f32<64>, grid, block, 0, stream, a, t);
+  else
+    hipLaunchKernelGGL(paged_tree_f32<128>, grid, block, 0, stream, a, t);
   return status_from_hip(hipGetLastError());
 }
 

@@ -47,6 +47,25 @@ struct DecodeArgs {
   int max_q_len;
 };
 
+// Drafted trees: node i of sequence s (packed row cu_q[s] + i) sees its sequence's ctx_start[s] cached keys and the
+// nodes e whose bits are set in its row of the mask. Key ranges of part_tokens keys: blockIdx.z of the grid, records
+// as for decode partitions with the packed row as the sequence.
+struct TreeMask {
+  const uint64_t* mask;
+  int64_t stride;  // words
+  int words;
+};
+
+// The keys key0 .. key0 + 31 that a mask row names, as bits; e0: tree number of key0 (below 0: cached, all set).
+__device__ __forceinline__ uint32_t tree_window(const uint64_t* row, int words, int e0) {
+  if (e0 <= -32) return 0xffffffffu;
+  if (e0 < 0) return static_cast<uint32_t>(row[0] << -e0) | ((1u << -e0) - 1u);
+  const int word = e0 >> 6, off = e0 & 63;
+  uint64_t x = word < words ? row[word] >> off : 0;
+  if (off > 32 && word + 1 < words) x |= row[word + 1] << (64 - off);
+  return static_cast<uint32_t>(x);
+}
+
 // The step's new K/V rows, appended by the stream kernel itself (mip_paged_decode_append).
 // slots == nullptr: no append.
 struct AppendRows {
@@ -219,6 +238,8 @@ int stream_max_pieces_env();
 using KernelFn = void (*)(DecodeArgs);
 KernelFn f32_decode_kernel(int d);
 int f32_prefill_launch(const DecodeArgs& a, int num_seqs, int d, hipStream_t stream);
+// Drafted trees, any group: a.nparts key ranges (records in a.ws_ml / a.ws_acc where there are several).
+int f32_tree_launch(const DecodeArgs& a, const TreeMask& t, int num_seqs, int d, hipStream_t stream);
 
 // Packed prefill attention for the shapes the 16-bit MFMA prefill kernel does not cover: fp32 at
 // head_dim 64 / 128 and up to 16 query heads per kv head on the fp32 matrix-core kernel where it

@@ -223,16 +223,8 @@ struct Rows {
   }
 };
 
-// The nodes among keys key0 .. key0 + 31 that a mask row names, as bits; cached keys (below ctx) are all set.
 __device__ __forceinline__ uint32_t mask_window(const TreeArgs& a, const Piece& p, int tok, int key0) {
-  const int e0 = key0 - p.q.ctx;  // tree number of the first key (below 0: cached)
-  if (e0 <= -32) return 0xffffffffu;
-  const uint64_t* row = a.mask + (static_cast<int64_t>(p.q.q0) + tok) * a.mask_st;
-  if (e0 < 0) return static_cast<uint32_t>(row[0] << -e0) | ((1u << -e0) - 1u);
-  const int word = e0 >> 6, off = e0 & 63;
-  uint64_t x = word < a.mask_words ? row[word] >> off : 0;
-  if (off > 32 && word + 1 < a.mask_words) x |= row[word + 1] << (64 - off);
-  return static_cast<uint32_t>(x);
+  return decode::tree_window(a.mask + (static_cast<int64_t>(p.q.q0) + tok) * a.mask_st, a.mask_words, key0 - p.q.ctx);
 }
 
 // Scores of 32 keys against a wavefront's rows, masked, and the rows' maxima brought up to date. k: the K operand of
@@ -931,8 +923,16 @@ __global__ __launch_bounds__(256) void paged_tree_merge(TreeArgs a, int segs_per
 // takes 64 / LPR keys at once and every key's row lanes keep a softmax state of their own (a score is summed
 // over its LPR lanes alone); the states meet at the end. A key that the row does not see contributes
 // nothing at all, whatever its bytes are.
+// Long contexts of few rows are cut into parts of `tokens` keys (blockIdx.z), which leave their states in
+// ml [row][head][part][2] and acc [row][head][part][D].
+struct PartArgs {
+  int hq, tokens, parts;
+  float* ml;
+  float* acc;
+};
+
 template <int DT, int D>
-__global__ __launch_bounds__(256) void paged_tree_row_kernel(TreeArgs a, int hq) {
+__global__ __launch_bounds__(256) void paged_tree_row_kernel(TreeArgs a, PartArgs pt) {
   using S = typename Elem<DT>::S;
   constexpr int ES = Elem<DT>::kBytes, N = 16 / ES, LPR = D / N > 0 ? D / N : 1, RPP = kWave / LPR;
   static_assert(D % N == 0 && LPR <= kWave, "a row is whole 16-byte chunks, at most 64");
@@ -943,7 +943,9 @@ __global__ __launch_bounds__(256) void paged_tree_row_kernel(TreeArgs a, int hq)
   const int s = static_cast<int>(x / a.max_q_len), i = static_cast<int>(x - static_cast<int64_t>(s) * a.max_q_len);
   const Seq p = seq_of(a, s);
   if (i >= p.n) return;
-  const int keys = keys_of(a, p);
+  const int all = keys_of(a, p), np = (all + pt.tokens - 1) / pt.tokens, part = blockIdx.z;
+  if (part >= np) return;
+  const int first = part * pt.tokens, keys = first + pt.tokens < all ? first + pt.tokens : all;
   const int h = blockIdx.y, kvh = h / a.group;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), w = tid / kWave;
   const int row = lane / LPR, c = lane % LPR;
@@ -972,8 +974,8 @@ __global__ __launch_bounds__(256) void paged_tree_row_kernel(TreeArgs a, int hq)
       if (in[u] && e0 >= 0) in[u] = (e0 >> 6) < a.mask_words && ((mask[e0 >> 6] >> (e0 & 63)) & 1u);
     }
   };
-  lookup(0);
-  for (int base = 0; base < keys; base += STEP) {
+  lookup(first);
+  for (int base = first; base < keys; base += STEP) {
     u32x4_t kw[U], vw[U];
     bool seen[U];
 #pragma unroll
@@ -1023,8 +1025,42 @@ __global__ __launch_bounds__(256) void paged_tree_row_kernel(TreeArgs a, int hq)
       A = fmaf(f, s_acc[k][d], A);
       Ls = fmaf(f, s_l[k], Ls);
     }
+    if (np == 1) {
+      reinterpret_cast<S*>(a.out)[r * a.out_st + static_cast<int64_t>(h) * a.out_sh + d] =
+          from_f32<DT>(Ls == 0.0f ? 0.0f : A / Ls);
+    } else {
+      const int64_t slot = (r * pt.hq + h) * pt.parts + part;
+      pt.acc[slot * D + d] = A;
+      if (d == 0) {
+        pt.ml[2 * slot] = top;
+        pt.ml[2 * slot + 1] = Ls;
+      }
+    }
+  }
+}
+
+// Combine the parts of every (node, query head) that has more than one: a wavefront each.
+template <int DT>
+__global__ __launch_bounds__(kWave) void paged_tree_parts_kernel(TreeArgs a, PartArgs pt, int dim) {
+  using S = typename Elem<DT>::S;
+  const int64_t x = blockIdx.x;  // (sequence, node)
+  const int s = static_cast<int>(x / a.max_q_len), i = static_cast<int>(x - static_cast<int64_t>(s) * a.max_q_len);
+  const Seq p = seq_of(a, s);
+  const int h = blockIdx.y, np = (keys_of(a, p) + pt.tokens - 1) / pt.tokens;
+  if (i >= p.n || np < 2) return;
+  const int64_t r = static_cast<int64_t>(p.q0) + i, slot = (r * pt.hq + h) * pt.parts;
+  float m = -INFINITY;
+  for (int k = 0; k < np; ++k) m = fmax2(m, pt.ml[2 * (slot + k)]);
+  for (int d = threadIdx.x; d < dim; d += kWave) {
+    float A = 0.0f, l = 0.0f;
+#pragma unroll 4
+    for (int k = 0; k < np; ++k) {
+      const float mk = pt.ml[2 * (slot + k)], f = mk == -INFINITY ? 0.0f : fast_exp2(mk - m);
+      A = fmaf(f, pt.acc[(slot + k) * dim + d], A);
+      l = fmaf(f, pt.ml[2 * (slot + k) + 1], l);
+    }
     reinterpret_cast<S*>(a.out)[r * a.out_st + static_cast<int64_t>(h) * a.out_sh + d] =
-        from_f32<DT>(Ls == 0.0f ? 0.0f : A / Ls);
+        from_f32<DT>(l == 0.0f ? 0.0f : A / l);
   }
 }
 
@@ -1032,6 +1068,7 @@ __global__ __launch_bounds__(256) void paged_tree_row_kernel(TreeArgs a, int hq)
 
 using KernelFn = void (*)(TreeArgs);
 using MergeFn = void (*)(TreeArgs, int, int);
+using KernelRowFn = void (*)(TreeArgs, PartArgs);
 
 struct Config {
   KernelFn fn = nullptr;
@@ -1116,21 +1153,52 @@ Plan plan_of(int num_seqs, int max_q_len, int hq, int hkv, int d, int bs, int ma
 // 14q/2kv d64: 1 x 5 over 60 keys 4.4/7.2, 500 8.9/10.3, 1000 14.6/11.0; 1 x 64 120 6.9/13.0, 500 13.5/14.4;
 // 32 x 5 16 6.4/8.0, 120 8.8/8.1; 8 x 24 60 9.1/13.9, 250 16.6/15.7; 28q/4kv d128: 1 x 5 250 8.6/12.5, 500 14.6/12.8;
 // 8 x 5 120 9.0/9.8, 250 14.4/13.6; 32 x 5 16 13.7/9.9).
-bool row_kernel_pays(int num_seqs, int max_q_len, int hq, int d, int64_t cap) {
-  const int64_t rows = static_cast<int64_t>(num_seqs) * max_q_len * hq;
-  return cap * d <= 49152 && rows * cap * d <= (int64_t{1} << 24);
+// In fp32 the tiles are the smaller ones and win earlier (1 x 5 over 60 keys 5.3/6.4, 8 x 7 over 16-256 9.0/8.5).
+bool row_kernel_pays(int num_seqs, int max_q_len, int hq, int d, int64_t cap, int dtype) {
+  const int64_t work = static_cast<int64_t>(num_seqs) * max_q_len * hq * cap * d;
+  return dtype == MIP_F32 ? cap * d <= 8192 && work <= (int64_t{1} << 22) : cap * d <= 49152 && work <= (int64_t{1} << 24);
+}
+
+// Parts of the other kernels' calls, at least kPartTokens keys each, where their workgroups leave half of the chip idle
+// (fp32, graph replay, us, whole / parts: 14 tiles of workgroups over 1000 keys 22.3/11.5, 2 over 2000 37.9/10.6, 32 over
+// 500 14.1/11.0; parts of 224 over 500 16.1/20.9).
+constexpr int kPartTokens = 256;
+struct Parts {
+  int tokens = 1, parts = 1;
+  int64_t acc_off = 0, bytes = 0;  // bytes 0: one part
+};
+
+Parts parts_of(int num_seqs, int max_q_len, int hq, int hkv, int d, int64_t cap, bool tiles) {
+  Parts p;
+  const int64_t rows = static_cast<int64_t>(num_seqs) * max_q_len, per_kv = static_cast<int64_t>(max_q_len) * (hq / hkv);
+  const int64_t groups = tiles ? (per_kv + 15) / 16 * hkv * num_seqs : rows * hq;
+  const int64_t want = groups < 256 ? 256 / groups : 1, most = (cap + kPartTokens - 1) / kPartTokens;
+  const int64_t parts = want < most ? want : most;
+  p.tokens = static_cast<int>(((cap + parts - 1) / parts + 63) / 64 * 64);
+  p.parts = static_cast<int>((cap + p.tokens - 1) / p.tokens);
+  if (p.parts > 1) {
+    p.acc_off = (rows * hq * p.parts * 8 + 255) / 256 * 256;
+    p.bytes = p.acc_off + rows * hq * p.parts * d * 4;
+  }
+  return p;
+}
+
+// fp32 on the matrix cores: head_dim 64 / 128, where its grid and its 32-bit pool rows suffice.
+bool f32_fits(int dtype, int d, int num_seqs, int64_t rows, int64_t pool_rows) {
+  return dtype == MIP_F32 && (d == 64 || d == 128) && (rows + 15) / 16 * num_seqs < (int64_t{1} << 24) &&
+         pool_rows < (int64_t{1} << 31);
 }
 
 template <int DT>
-bool launch_row_d(const TreeArgs& a, int d, int hq, dim3 grid, hipStream_t s) {
+KernelRowFn row_kernel(int d) {
   switch (d) {
-    case 8:   hipLaunchKernelGGL((paged_tree_row_kernel<DT, 8>), grid, dim3(256), 0, s, a, hq); return true;
-    case 16:  hipLaunchKernelGGL((paged_tree_row_kernel<DT, 16>), grid, dim3(256), 0, s, a, hq); return true;
-    case 32:  hipLaunchKernelGGL((paged_tree_row_kernel<DT, 32>), grid, dim3(256), 0, s, a, hq); return true;
-    case 64:  hipLaunchKernelGGL((paged_tree_row_kernel<DT, 64>), grid, dim3(256), 0, s, a, hq); return true;
-    case 128: hipLaunchKernelGGL((paged_tree_row_kernel<DT, 128>), grid, dim3(256), 0, s, a, hq); return true;
-    case 256: hipLaunchKernelGGL((paged_tree_row_kernel<DT, 256>), grid, dim3(256), 0, s, a, hq); return true;
-    default:  return false;
+    case 8:   return paged_tree_row_kernel<DT, 8>;
+    case 16:  return paged_tree_row_kernel<DT, 16>;
+    case 32:  return paged_tree_row_kernel<DT, 32>;
+    case 64:  return paged_tree_row_kernel<DT, 64>;
+    case 128: return paged_tree_row_kernel<DT, 128>;
+    case 256: return paged_tree_row_kernel<DT, 256>;
+    default:  return nullptr;
   }
 }
 
@@ -1147,8 +1215,16 @@ extern "C" size_t mip_paged_tree_workspace(int32_t num_seqs, int32_t max_q_len, 
       head_dim <= 0 || block_size <= 0 || max_blocks_per_seq <= 0 ||
       static_cast<int64_t>(max_blocks_per_seq) * block_size >= (int64_t{1} << 30))
     return 0;
-  return static_cast<size_t>(
-      tree::plan_of(num_seqs, max_q_len, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, dtype).bytes);
+  const int64_t cap = static_cast<int64_t>(max_blocks_per_seq) * block_size;
+  // The larger of what the kernels need that may take the call (its alignment is not known here).
+  const int64_t main =
+      tree::plan_of(num_seqs, max_q_len, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, dtype).bytes;
+  int64_t need = main;
+  for (const bool tiles : {false, dtype == MIP_F32}) {
+    const int64_t rest = tree::parts_of(num_seqs, max_q_len, num_heads, num_kv_heads, head_dim, cap, tiles).bytes;
+    need = rest > need ? rest : need;
+  }
+  return static_cast<size_t>(need);
 }
 
 extern "C" int mip_paged_tree(void* out, int64_t out_stride_tok, int64_t out_stride_head, const void* q,
@@ -1208,7 +1284,7 @@ extern "C" int mip_paged_tree(void* out, int64_t out_stride_tok, int64_t out_str
                            ? tree::Plan{}
                            : tree::plan_of(num_seqs, max_q_len, num_heads, num_kv_heads, head_dim, block_size,
                                            max_blocks_per_seq, dtype);
-  if (p.ok && !tree::row_kernel_pays(num_seqs, max_q_len, num_heads, head_dim, cap)) {
+  if (p.ok && !tree::row_kernel_pays(num_seqs, max_q_len, num_heads, head_dim, cap, dtype)) {
     if (p.bytes > 0) {
       if (!workspace || workspace_bytes < static_cast<size_t>(p.bytes) || (reinterpret_cast<uintptr_t>(workspace) & 255))
         return MIP_EINVAL;
@@ -1231,12 +1307,60 @@ extern "C" int mip_paged_tree(void* out, int64_t out_stride_tok, int64_t out_str
   }
   const int64_t rows = static_cast<int64_t>(num_seqs) * max_q_len;
   if (rows >= (int64_t{1} << 24) || num_heads > 65535) return MIP_EUNSUPPORTED;
-  const dim3 grid(static_cast<unsigned>(rows), num_heads);
-  bool found;
-  switch (dtype) {
-    case MIP_F32: found = tree::launch_row_d<MIP_F32>(a, head_dim, num_heads, grid, s); break;
-    case MIP_F16: found = tree::launch_row_d<MIP_F16>(a, head_dim, num_heads, grid, s); break;
-    default:      found = tree::launch_row_d<MIP_BF16>(a, head_dim, num_heads, grid, s); break;
+  const bool tiles = tree::f32_fits(dtype, head_dim, num_seqs, static_cast<int64_t>(max_q_len) * a.group,
+                                    num_cache_blocks * num_kv_heads * block_size) &&
+                     !tree::row_kernel_pays(num_seqs, max_q_len, num_heads, head_dim, cap, dtype);
+  const tree::KernelRowFn fn = dtype == MIP_F32   ? tree::row_kernel<MIP_F32>(head_dim)
+                               : dtype == MIP_F16 ? tree::row_kernel<MIP_F16>(head_dim)
+                                                  : tree::row_kernel<MIP_BF16>(head_dim);
+  if (!fn) return MIP_EUNSUPPORTED;
+  const tree::Parts parts = tree::parts_of(num_seqs, max_q_len, num_heads, num_kv_heads, head_dim, cap, tiles);
+  tree::PartArgs pt{num_heads, parts.tokens, parts.parts, nullptr, nullptr};
+  if (parts.bytes > 0) {
+    if (!workspace || workspace_bytes < static_cast<size_t>(parts.bytes) || (reinterpret_cast<uintptr_t>(workspace) & 255))
+      return MIP_EINVAL;
+    pt.ml = static_cast<float*>(workspace);
+    pt.acc = reinterpret_cast<float*>(static_cast<char*>(workspace) + parts.acc_off);
   }
-  return found ? status_from_hip(hipGetLastError()) : MIP_EUNSUPPORTED;
+  if (tiles) {
+    decode::DecodeArgs da{};
+    da.out = a.out;
+    da.out_sb = out_stride_tok;
+    da.out_sh = out_stride_head;
+    da.q = a.q;
+    da.q_sb = q_stride_tok;
+    da.q_sh = q_stride_head;
+    da.k = a.k;
+    da.v = a.v;
+    da.ncb = num_cache_blocks;
+    da.bt = block_tables;
+    da.bt_stride = bt_stride;
+    da.hq = num_heads;
+    da.hkv = num_kv_heads;
+    da.bs = block_size;
+    da.log2_bs = a.log2_bs;
+    da.max_blocks = max_blocks_per_seq;
+    da.group = a.group;
+    da.part_tokens = parts.tokens;
+    da.nparts = parts.parts;
+    da.scale_log2 = a.scale_log2;
+    da.ws_ml = pt.ml;
+    da.ws_acc = pt.acc;
+    da.cu_q = cu_q;
+    da.ctx_start = ctx_start;
+    da.max_q_len = max_q_len;
+    const int st = decode::f32_tree_launch(da, decode::TreeMask{mask, mask_stride, mask_words}, num_seqs, head_dim, s);
+    if (st) return st;
+  } else {
+    hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(rows), num_heads, parts.parts), dim3(256), 0, s, a, pt);
+  }
+  if (parts.parts > 1) {
+    const dim3 grid(static_cast<unsigned>(rows), num_heads);
+    switch (dtype) {
+      case MIP_F32: hipLaunchKernelGGL(tree::paged_tree_parts_kernel<MIP_F32>, grid, dim3(kWave), 0, s, a, pt, head_dim); break;
+      case MIP_F16: hipLaunchKernelGGL(tree::paged_tree_parts_kernel<MIP_F16>, grid, dim3(kWave), 0, s, a, pt, head_dim); break;
+      default:      hipLaunchKernelGGL(tree::paged_tree_parts_kernel<MIP_BF16>, grid, dim3(kWave), 0, s, a, pt, head_dim);
+    }
+  }
+  return status_from_hip(hipGetLastError());
 }

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from functools import lru_cache
 from itertools import chain
 
 import numpy as np
@@ -737,7 +738,8 @@ def _one_device(*tensors: torch.Tensor) -> torch.device:
     for t in tensors:
         if t.device != device:
             raise ValueError(f"tensors on different devices: {device} and {t.device}")
-    _require_device(tensors[0])
+    if device.type != "cuda":
+        _require_device(tensors[0])
     return device
 
 
@@ -785,6 +787,17 @@ def _scratch(workspace: torch.Tensor | None, device: torch.device, need: int) ->
     return workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
+@lru_cache(4096)
+def _tree_bytes(device: torch.device, *shape) -> int:
+    with torch.cuda.device(device):  # the size follows the current device
+        return int(_native.load().mip_paged_tree_workspace(*shape))
+
+
+@lru_cache(4096)
+def _verify_bytes(*shape) -> int:
+    return int(_native.load().mip_tree_verify_workspace(*shape))
+
+
 def tree_index(parents: torch.Tensor, cu_q: torch.Tensor, ctx_start: torch.Tensor, block_tables: torch.Tensor,
                max_q_len: int, block_size: int,
                max_blocks: int | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -803,9 +816,8 @@ def tree_index(parents: torch.Tensor, cu_q: torch.Tensor, ctx_start: torch.Tenso
         raise ValueError("parents must be contiguous int32 [N]")
     device = _one_device(parents, cu_q, ctx_start, block_tables)
     n, words = parents.shape[0], (max_q_len + 63) // 64
-    both = torch.empty(2 * n, dtype=torch.int64, device=device)
-    mask = torch.empty(n, words, dtype=torch.int64, device=device)
-    positions, slots = both[:n], both[n:]
+    positions = torch.empty(n, dtype=torch.int64, device=device)
+    slots, mask = torch.empty_like(positions), positions.new_empty(n, words)
     if n and s and max_q_len:
         _call_on(device, _native.load().mip_tree_index,
                  (positions.data_ptr(), slots.data_ptr(), mask.data_ptr(), words, parents.data_ptr(), cu_q.data_ptr(),
@@ -851,14 +863,14 @@ def paged_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
     if not scale > 0.0:
         raise ValueError(f"scale={scale} must be positive")
     if out is None:
-        out = torch.empty((n, hq, d), dtype=q.dtype, device=q.device)
+        out = q.new_empty(n, hq, d)
     elif out.shape != (n, hq, d) or out.dtype != q.dtype or out.stride(2) != 1:
         raise ValueError("out must be [N, Hq, D] in q's dtype with a contiguous last dimension")
     device = _one_device(q, k_cache, v_cache, block_tables, cu_q, ctx_start, mask, out)
     if not (n and s and max_q_len):
         return out
     code, lib = dtype_code(q.dtype), _native.load()
-    ws_ptr, ws_bytes = _scratch(workspace, device, int(lib.mip_paged_tree_workspace(s, max_q_len, hq, hkv, d, bs, mb, code)))
+    ws_ptr, ws_bytes = _scratch(workspace, device, _tree_bytes(device, s, max_q_len, hq, hkv, d, bs, mb, code))
     _call_on(device, lib.mip_paged_tree,
              (out.data_ptr(), out.stride(0), out.stride(1), q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
               v_cache.data_ptr(), nb, block_tables.data_ptr(), block_tables.stride(0), cu_q.data_ptr(),
@@ -869,7 +881,8 @@ def paged_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
 
 def tree_workspace_bytes(num_seqs: int, max_q_len: int, num_heads: int, num_kv_heads: int, head_dim: int,
                          block_size: int, max_blocks: int, dtype: torch.dtype) -> int:
-    """Bytes of scratch a :func:`paged_tree` call of this shape needs (``mip_paged_tree_workspace``)."""
+    """Bytes of scratch a :func:`paged_tree` call of this shape needs on the current device
+    (``mip_paged_tree_workspace``)."""
     return int(_native.load().mip_paged_tree_workspace(num_seqs, max_q_len, num_heads, num_kv_heads, head_dim,
                                                        block_size, max_blocks, dtype_code(dtype)))
 
@@ -902,13 +915,11 @@ def tree_verify(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
     s, row_stride = cu_q.shape[0] - 1, max(logits.stride(0), vocab) if n <= 1 else logits.stride(0)
     if row_stride < vocab:
         raise ValueError("the rows of logits overlap")
-    both = torch.empty(n + s, dtype=torch.int64, device=device)
-    ints = torch.empty(s * max_q_len + s, dtype=torch.int32, device=device)
-    target, following = both[:n], both[n:]
-    path, counts = ints[:s * max_q_len].view(s, max_q_len), ints[s * max_q_len:]
+    target, following = torch.empty_like(tokens), tokens.new_empty(s)
+    path, counts = cu_q.new_empty(s, max_q_len), cu_q.new_empty(s)
     if n or s:
         lib = _native.load()
-        ws_ptr, ws_bytes = _scratch(workspace, device, int(lib.mip_tree_verify_workspace(n, vocab, code)))
+        ws_ptr, ws_bytes = _scratch(workspace, device, _verify_bytes(n, vocab, code))
         _call_on(device, lib.mip_tree_verify,
                  (target.data_ptr(), path.data_ptr(), counts.data_ptr(), following.data_ptr(), logits.data_ptr(),
                   row_stride, n, vocab, tokens.data_ptr(), parents.data_ptr(), cu_q.data_ptr(), s, max_q_len, ws_ptr,
