@@ -540,6 +540,20 @@ typedef struct mip_prefill_step {
   float scale;
 } mip_prefill_step;
 
+typedef struct mip_tree_step {
+  int64_t out_stride_tok, out_stride_head, q_stride_tok, q_stride_head, num_cache_blocks;
+  const int32_t* block_tables;
+  int64_t bt_stride;
+  const int32_t* cu_q;
+  const int32_t* ctx_start;
+  const uint64_t* mask;
+  int64_t mask_stride;
+  void* workspace;
+  size_t workspace_bytes;
+  int32_t mask_words, num_seqs, max_q_len, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, dtype;
+  float scale;
+} mip_tree_step;
+
 /* mip_paged_decode_append */
 int mip_decode_step_append(const mip_decode_step* step, const void* k_new, const void* v_new, void* out,
                            const void* q, void* k_cache, void* v_cache, void* stream);
@@ -554,6 +568,9 @@ int mip_prefill_step_append(const mip_prefill_step* step, const void* k_new, con
                             void* v_cache, void* stream);
 int mip_prefill_step_attend(const mip_prefill_step* step, void* out, const void* q, const void* k_cache,
                             const void* v_cache, void* stream);
+/* mip_paged_tree (the nodes are appended with mip_prefill_step_append / mip_rope_step_append) */
+int mip_tree_step_attend(const mip_tree_step* step, void* out, const void* q, const void* k_cache, const void* v_cache,
+                         void* stream);
 
 #ifdef __cplusplus
 }

@@ -52,3 +52,13 @@ extern "C" int mip_prefill_step_attend(const mip_prefill_step* s, void* out, con
                            s->num_seqs, s->max_q_len, s->num_heads, s->num_kv_heads, s->head_dim, s->block_size,
                            s->max_blocks_per_seq, s->scale, s->dtype, stream);
 }
+
+extern "C" int mip_tree_step_attend(const mip_tree_step* s, void* out, const void* q, const void* k_cache,
+                                    const void* v_cache, void* stream) {
+  if (!s) return MIP_EINVAL;
+  return mip_paged_tree(out, s->out_stride_tok, s->out_stride_head, q, s->q_stride_tok, s->q_stride_head, k_cache, v_cache,
+                        s->num_cache_blocks, s->block_tables, s->bt_stride, s->cu_q, s->ctx_start, s->mask,
+                        s->mask_stride, s->mask_words, s->num_seqs, s->max_q_len, s->num_heads, s->num_kv_heads,
+                        s->head_dim, s->block_size, s->max_blocks_per_seq, s->scale, s->workspace, s->workspace_bytes,
+                        s->dtype, stream);
+}

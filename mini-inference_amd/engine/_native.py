@@ -52,6 +52,7 @@ EXPORTED = (
     "mip_tree_verify",
     "mip_tree_verify_workspace",
     "mip_tree_commit",
+    "mip_tree_step_attend",
 )
 
 # Measurement helpers in the same library (include/mipaged_probe.h), outside the drop-in ABI.
@@ -89,6 +90,17 @@ class PrefillStep(_c.Structure):
                                                       "q_stride_head", "num_cache_blocks")] + [
         ("block_tables", _vp), ("bt_stride", _i64), ("cu_q", _vp), ("ctx_start", _vp)] + [
         (n, _i32) for n in ("n_tokens", "num_seqs", "max_q_len", "num_heads", "num_kv_heads", "head_dim", "block_size",
+                            "max_blocks_per_seq", "dtype")] + [("scale", _f32)]
+
+
+class TreeStep(_c.Structure):
+    """``mip_tree_step``: what every layer's tree attention call of one step shares."""
+
+    _fields_ = [(n, _i64) for n in ("out_stride_tok", "out_stride_head", "q_stride_tok", "q_stride_head",
+                                    "num_cache_blocks")] + [
+        ("block_tables", _vp), ("bt_stride", _i64), ("cu_q", _vp), ("ctx_start", _vp), ("mask", _vp),
+        ("mask_stride", _i64), ("workspace", _vp), ("workspace_bytes", _sz)] + [
+        (n, _i32) for n in ("mask_words", "num_seqs", "max_q_len", "num_heads", "num_kv_heads", "head_dim", "block_size",
                             "max_blocks_per_seq", "dtype")] + [("scale", _f32)]
 
 
@@ -138,6 +150,7 @@ _SIGNATURES = {
     "mip_rope_step_append": (_c.c_int, [_vp] * 9),
     "mip_prefill_step_append": (_c.c_int, [_vp] * 6),
     "mip_prefill_step_attend": (_c.c_int, [_vp] * 6),
+    "mip_tree_step_attend": (_c.c_int, [_vp] * 6),
     "mip_decode_prepare": (_c.c_int, [_vp, _i64, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _i32, _vp, _vp, _i32, _i32, _vp]),
     "mip_rope_tables": (_c.c_int, [_vp, _vp, _vp, _i32, _i32, _f32, _i32, _vp]),
     "mip_prefill_index": (_c.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp]),

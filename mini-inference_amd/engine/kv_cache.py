@@ -12,6 +12,8 @@ Drop-in for the paged half of the reference's engine/kv_cache.py:
   batch's slot ids, positions and the table entries written since the last step.
 * :class:`PackedPrefillContext` (engine/kv_cache.py:218-301): the packed scatter is the
   append kernel and the attention over cached prefixes is the paged prefill kernel.
+* :class:`PagedTreeContext` (no reference counterpart): a step of speculative decoding, which
+  verifies a tree of drafted tokens per sequence in one pass.
 
 Pool layout (reference engine/kv_cache.py:426-428):
 ``k, v: [num_layers, num_blocks + 1, num_kv_heads, block_size, head_dim]``; block
@@ -311,6 +313,10 @@ class PagedKVCache:
 
     def decode_context(self, slots: Sequence[int]) -> "PagedDecodeContext":
         return PagedDecodeContext(self, slots)
+
+    def tree_context(self, slots: Sequence[int], tokens: Sequence[Sequence[int]],
+                     parents: Sequence[Sequence[int]]) -> "PagedTreeContext":
+        return PagedTreeContext(self, slots, tokens, parents)
 
 
 class DeviceBlockTables:
@@ -639,3 +645,137 @@ class PackedPrefillContext:
     def commit(self) -> None:
         for slot, start, n in zip(self.slots, self.starts, self.lengths):
             self.cache.lengths[slot] = start + n
+
+
+class PagedTreeContext:
+    """A step of speculative decoding: a tree of drafted tokens per sequence, verified in one pass of the model.
+
+    ``tokens[s]`` are the tokens of sequence s's nodes and ``parents[s]`` each node's parent by its number in the tree.
+    Node 0, the root (parent -1), is the sequence's last token, which is not cached yet (what a decode step would be
+    given); every other node is a drafted token that continues a node before it. No reference counterpart: the
+    reference decodes one token a step (engine/kv_cache.py:582-624).
+
+    Run the model on ``input_ids`` and ``positions`` (int64 ``[N]``, the trees packed end to end), compute the logits of
+    all N rows and hand them to :meth:`accept`::
+
+        ctx = cache.tree_context(slots, tokens, parents)
+        hidden = model(ctx.input_ids.unsqueeze(0), ctx.positions.unsqueeze(0), ctx)
+        new_tokens = ctx.accept(model.compute_logits(hidden[0]))
+
+    Node i is stored behind the cached tokens in its own place (``slot_mapping``), whatever its depth, and sees the cached
+    tokens and its own path (``mask``); accepting a path moves its rows to consecutive places. The blocks for all
+    nodes are allocated, and shared ones copied, when the context is made; those that the accepted path does not fill
+    stay with the sequence for its next tokens.
+    """
+
+    fuse_rope = True
+
+    def __init__(self, cache: PagedKVCache, slots: Sequence[int], tokens: Sequence[Sequence[int]],
+                 parents: Sequence[Sequence[int]]) -> None:
+        self.cache = cache
+        self.slots = list(slots)
+        if not self.slots:
+            raise ValueError("a tree step needs at least one sequence")
+        if len(set(self.slots)) != len(self.slots):
+            raise ValueError("a sequence occurs twice in one tree step")
+        if len(tokens) != len(self.slots) or len(parents) != len(self.slots):
+            raise ValueError(f"{len(self.slots)} sequences, but {len(tokens)} lists of tokens and {len(parents)} of parents")
+        for toks, tree in zip(tokens, parents):
+            if not len(toks) == len(tree) or not len(tree):
+                raise ValueError("every tree needs a root, and a token and a parent for each node")
+            if tree[0] != -1 or any(not 0 <= p < i for i, p in enumerate(tree) if i):
+                raise ValueError("node 0 is the root (parent -1) and every other node's parent comes before it")
+        self.lengths = [len(t) for t in tokens]
+        self.max_q_len = max(self.lengths)
+        if self.max_q_len > paged_ops.MAX_TREE_NODES:
+            raise ValueError(f"a tree of {self.max_q_len} nodes; at most {paged_ops.MAX_TREE_NODES}")
+        paged_ops._require_device(cache.k)
+        self.tokens = [list(t) for t in tokens]
+        self.starts = [cache.lengths[s] for s in self.slots]
+        ends = [a + n for a, n in zip(self.starts, self.lengths)]
+        for s, end in zip(self.slots, ends):
+            if not cache.ensure_capacity(s, end):
+                raise ValueError(f"no room in the KV cache for {end} tokens")
+        cache.prepare_writes(self.slots, self.starts, self.lengths)
+        dev = cache.k.device
+        s_n, n, nb = len(self.slots), sum(self.lengths), max(1, cache.blocks_for(max(ends)))
+        # One upload: tokens (int64) | row offsets | cached lengths | parents | tables (int32).
+        n32 = 2 * s_n + 1 + n + s_n * nb
+        host = torch.empty(n + (n32 + 1) // 2, dtype=torch.int64, pin_memory=dev.type == "cuda")
+        host.numpy()[:n] = np.fromiter(chain.from_iterable(self.tokens), dtype=np.int64, count=n)
+        i32 = host.numpy()[n:].view(np.int32)
+        i32[0] = 0
+        np.cumsum(self.lengths, out=i32[1:s_n + 1])
+        i32[s_n + 1:2 * s_n + 1] = self.starts
+        at = 2 * s_n + 1
+        i32[at:at + n] = np.fromiter(chain.from_iterable(parents), dtype=np.int32, count=n)
+        tables = i32[at + n:n32].reshape(s_n, nb)
+        tables.fill(0)
+        for row, s in zip(tables, self.slots):
+            ids = cache.block_tables[s][:nb]
+            row[:len(ids)] = ids
+        i32[n32:] = 0
+        on_dev = host.to(dev, non_blocking=True)
+        self.input_ids, d32 = on_dev[:n], on_dev[n:].view(torch.int32)
+        self.cu_q, self.ctx_start, self.parents = d32[:s_n + 1], d32[s_n + 1:at], d32[at:at + n]
+        self.block_tables = d32[at + n:n32].view(s_n, nb)
+        self.positions, self.slot_mapping, self.mask = paged_ops.tree_index(
+            self.parents, self.cu_q, self.ctx_start, self.block_tables, self.max_q_len, cache.block_size)
+        # As for a packed prefill: in place when the constructor returns, on whatever stream it is used then.
+        torch.cuda.current_stream(dev).synchronize()
+        self._calls: paged_ops.TreeStepCalls | None = None
+        self._settled = False
+
+    @property
+    def calls(self) -> paged_ops.TreeStepCalls:
+        """The step's layer calls: the shared arguments are checked on the first layer only."""
+        if self._calls is None:
+            self._calls = paged_ops.TreeStepCalls(self.block_tables, self.cu_q, self.ctx_start, self.mask,
+                                                  self.slot_mapping, self.max_q_len, 1.0 / (self.cache.head_dim ** 0.5))
+        return self._calls
+
+    def attend(self, layer_idx: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
+        """Append the nodes' k/v, then attend; q, k, v ``[1, H, N, D]`` after the rotary embedding."""
+        calls, c = self.calls, self.cache
+        calls.append(layer_idx, k, v, c.k, c.v)
+        return calls.attend(layer_idx, q, c.k, c.v)
+
+    def attend_rope(self, layer_idx: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor,
+                    sin: torch.Tensor) -> torch.Tensor:
+        """:meth:`attend` on pre-rotation q and k, the rotation fused into the append (``cos``, ``sin [1, 1, N, D]``)."""
+        calls, c = self.calls, self.cache
+        calls.rope_append(layer_idx, q, k, v, cos, sin, c.k, c.v)
+        return calls.attend(layer_idx, q, c.k, c.v)
+
+    def verify(self, logits: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+        """:func:`paged_ops.tree_verify` of this step's trees against the logits ``[N, vocab]`` of its rows."""
+        return paged_ops.tree_verify(logits, self.input_ids, self.parents, self.cu_q, self.max_q_len)
+
+    def accept(self, logits: torch.Tensor) -> list[list[int]]:
+        """Greedy verification: keep the longest path that the logits agree with; returns each sequence's new tokens.
+
+        Those are the path's drafted tokens and the model's token after them (one at least: what a decode step
+        would have returned). The root and the path's tokens are cached and counted from then on; the last new
+        token is not, and is the next step's root.
+        """
+        _, path, counts, following = self.verify(logits)
+        kept = self.commit(path, counts)
+        return [[ids[i] for i in nodes[1:]] + [token] for ids, nodes, token in zip(self.tokens, kept, following.tolist())]
+
+    def commit(self, path: torch.Tensor, counts: torch.Tensor) -> list[list[int]]:
+        """Keep the nodes ``path[s, :counts[s]]`` (node 0 first, each below a node before it): their rows are moved to
+        consecutive places and the sequences' lengths updated. Returns the paths. Once per step."""
+        if self._settled:
+            raise RuntimeError("this step's tokens have been committed")
+        nodes = [row[:k] for row, k in zip(path.tolist(), counts.tolist())]
+        if len(nodes) != len(self.slots):
+            raise ValueError(f"{len(nodes)} paths for {len(self.slots)} sequences")
+        for kept, n in zip(nodes, self.lengths):
+            if not kept or kept[0] != 0 or any(a >= b for a, b in zip(kept, kept[1:])) or kept[-1] >= n:
+                raise ValueError(f"not a path of nodes below {n} from the root on: {kept}")
+        if any(kept[-1] != len(kept) - 1 for kept in nodes):  # else every row is in place
+            paged_ops.tree_commit(self.cache.k, self.cache.v, self.block_tables, self.ctx_start, path, counts)
+        self._settled = True
+        for slot, start, kept in zip(self.slots, self.starts, nodes):
+            self.cache.lengths[slot] = start + len(kept)
+        return nodes

@@ -17,6 +17,8 @@ import torch
 
 from . import _native
 
+MAX_TREE_NODES = _native.MIP_TREE_MAX_NODES
+
 _DTYPE_CODES = {torch.float32: _native.MIP_F32, torch.float16: _native.MIP_F16, torch.bfloat16: _native.MIP_BF16}
 
 
@@ -826,24 +828,12 @@ def tree_index(parents: torch.Tensor, cu_q: torch.Tensor, ctx_start: torch.Tenso
     return positions, slots, mask
 
 
-def paged_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
-               cu_q: torch.Tensor, ctx_start: torch.Tensor, mask: torch.Tensor, max_q_len: int,
-               scale: float | None = None, out: torch.Tensor | None = None, max_blocks: int | None = None,
-               workspace: torch.Tensor | None = None) -> torch.Tensor:
-    """Attention of drafted trees' nodes over their sequences' paged keys and each other.
-
-    ``q``: ``[N, Hq, D]`` packed rows (last dim contiguous); sequence ``s`` owns rows ``cu_q[s] ..
-    cu_q[s + 1] - 1`` (int32 ``[S + 1]``), whose keys and values are in the pool at cache indexes
-    ``ctx_start[s] + i`` (int32 ``[S]``; append them first). A row sees its sequence's ``ctx_start[s]`` cached keys and
-    the nodes that its bits in ``mask`` (int64 ``[N, W]``, ``W >= ceil(max_q_len / 64)``, rows contiguous) name; a row that sees
-    nothing becomes zeros, and what a row does not see has no influence on it. Returns ``out [N, Hq, D]``; rows of no
-    sequence are not written. No reference counterpart (one token a step there, engine/kv_cache.py:615-620).
-
-    16-bit types at head_dim 64 / 128 run on the matrix cores, long contexts of few rows cut into pieces and
-    combined; other types and head sizes (powers of two from 8 to 256) one query row at a time. Scratch
-    memory is shared by the calls of a device, which must then be ordered; pass ``workspace``
-    (:func:`tree_workspace_bytes`) to calls that may run at once.
-    """
+def _tree_args(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+               cu_q: torch.Tensor, ctx_start: torch.Tensor, mask: torch.Tensor, max_q_len: int, scale: float | None,
+               out: torch.Tensor | None, max_blocks: int | None,
+               workspace: torch.Tensor | None) -> tuple[tuple | None, torch.Tensor, torch.Tensor | None]:
+    """Validate a :func:`paged_tree` call: the arguments of ``mip_paged_tree`` up to the stream (None for a call that
+    has nothing to do), the output and the scratch memory."""
     if q.dim() != 3 or q.stride(2) != 1:
         raise ValueError("q must be [N, Hq, D] with a contiguous last dimension")
     if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
@@ -860,7 +850,7 @@ def paged_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
             mask.shape[1] > 1 and mask.stride(1) != 1):
         raise ValueError(f"mask must be int64 [{n}, >= {words}] with contiguous rows, got {tuple(mask.shape)} {mask.dtype}")
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    if not scale > 0.0:
+    if not 0.0 < scale < math.inf:
         raise ValueError(f"scale={scale} must be positive")
     if out is None:
         out = q.new_empty(n, hq, d)
@@ -868,15 +858,74 @@ def paged_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
         raise ValueError("out must be [N, Hq, D] in q's dtype with a contiguous last dimension")
     device = _one_device(q, k_cache, v_cache, block_tables, cu_q, ctx_start, mask, out)
     if not (n and s and max_q_len):
-        return out
-    code, lib = dtype_code(q.dtype), _native.load()
-    ws_ptr, ws_bytes = _scratch(workspace, device, _tree_bytes(device, s, max_q_len, hq, hkv, d, bs, mb, code))
-    _call_on(device, lib.mip_paged_tree,
-             (out.data_ptr(), out.stride(0), out.stride(1), q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
-              v_cache.data_ptr(), nb, block_tables.data_ptr(), block_tables.stride(0), cu_q.data_ptr(),
-              ctx_start.data_ptr(), mask.data_ptr(), mask.stride(0), mask.shape[1], s, max_q_len, hq, hkv, d, bs, mb,
-              scale, ws_ptr, ws_bytes, code), "mip_paged_tree")
+        return None, out, None
+    code = dtype_code(q.dtype)
+    need = _tree_bytes(device, s, max_q_len, hq, hkv, d, bs, mb, code)
+    if workspace is None:
+        workspace = _workspace.get(device, need)
+    ws_ptr, ws_bytes = _scratch(workspace, device, need)
+    return (out.data_ptr(), out.stride(0), out.stride(1), q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
+            v_cache.data_ptr(), nb, block_tables.data_ptr(), block_tables.stride(0), cu_q.data_ptr(),
+            ctx_start.data_ptr(), mask.data_ptr(), mask.stride(0), mask.shape[1], s, max_q_len, hq, hkv, d, bs, mb,
+            scale, ws_ptr, ws_bytes, code), out, workspace
+
+
+def paged_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+               cu_q: torch.Tensor, ctx_start: torch.Tensor, mask: torch.Tensor, max_q_len: int,
+               scale: float | None = None, out: torch.Tensor | None = None, max_blocks: int | None = None,
+               workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of drafted trees' nodes over their sequences' paged keys and each other.
+
+    ``q``: ``[N, Hq, D]`` packed rows (last dim contiguous); sequence ``s`` owns rows ``cu_q[s] ..
+    cu_q[s + 1] - 1`` (int32 ``[S + 1]``), whose keys and values are in the pool at cache indexes
+    ``ctx_start[s] + i`` (int32 ``[S]``; append them first). A row sees its sequence's ``ctx_start[s]`` cached keys and
+    the nodes that its bits in ``mask`` (int64 ``[N, W]``, ``W >= ceil(max_q_len / 64)``, rows contiguous) name; a row that sees
+    nothing becomes zeros, and what a row does not see has no influence on it. Returns ``out [N, Hq, D]``; rows of no
+    sequence are not written. No reference counterpart (one token a step there, engine/kv_cache.py:615-620).
+
+    16-bit types at head_dim 64 / 128 run on the matrix cores, long contexts of few rows cut into pieces and
+    combined; fp32 at those head sizes on the fp32 matrix cores; other head sizes (powers of two from 8 to 256) and short
+    calls one query row at a time. Scratch memory is shared by the calls of a device, which must then be ordered; pass
+    ``workspace`` (:func:`tree_workspace_bytes`) to calls that may run at once.
+    """
+    args, out, _ = _tree_args(q, k_cache, v_cache, block_tables, cu_q, ctx_start, mask, max_q_len, scale, out, max_blocks,
+                              workspace)
+    if args is not None:
+        _call_on(q.device, _native.load().mip_paged_tree, args, "mip_paged_tree")
     return out
+
+
+class TreeStepCalls(PrefillStepCalls):
+    """The layer calls of one step of drafted trees; the nodes are appended as a packed prefill's tokens are."""
+
+    def __init__(self, block_tables: torch.Tensor, cu_q: torch.Tensor, ctx_start: torch.Tensor, mask: torch.Tensor,
+                 slot_mapping: torch.Tensor, max_q_len: int, scale: float) -> None:
+        super().__init__(block_tables, cu_q, ctx_start, slot_mapping, max_q_len, scale)
+        self.mask = mask
+
+    def attend(self, layer: int, q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor) -> torch.Tensor:
+        """:func:`paged_tree` of one layer; returns ``[1, Hq, N, D]``, a view of ``[N, Hq, D]``."""
+        key = (_layout(q), _layout(k_pool), _layout(v_pool))
+        hit = self._hit("attend", key, layer)
+        if hit is not None:
+            _, step, _, kb, vb, _, _ = hit
+            _, hq, n, d = q.shape
+            out = torch.empty_strided((1, hq, n, d), (hq * d, d, hq * d, 1), dtype=q.dtype, device=q.device)
+            _call_on(q.device, _native.load().mip_tree_step_attend,
+                     (step, out.data_ptr(), q.data_ptr(), k_pool.data_ptr() + layer * kb, v_pool.data_ptr() + layer * vb),
+                     "mip_tree_step_attend")
+            return out
+        q1 = q[0].transpose(0, 1)
+        a, out, workspace = _tree_args(q1, k_pool[layer], v_pool[layer], self.block_tables, self.cu_q, self.ctx_start,
+                                       self.mask, self.max_q_len, self.scale, None, None, None)
+        if a is not None:
+            _call_on(q.device, _native.load().mip_paged_tree, a, "mip_paged_tree")
+            if q.shape[0] == 1:
+                step = _native.TreeStep(a[1], a[2], a[4], a[5], a[8], a[9], a[10], a[11], a[12], a[13], a[14], a[24], a[25],
+                                        *a[15:23], a[26], a[23])
+                self._keep("attend", key, step, k_pool, v_pool, (self.block_tables, self.cu_q, self.ctx_start, self.mask,
+                                                                 workspace))
+        return out.transpose(0, 1).unsqueeze(0)
 
 
 def tree_workspace_bytes(num_seqs: int, max_q_len: int, num_heads: int, num_kv_heads: int, head_dim: int,
@@ -911,10 +960,10 @@ def tree_verify(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
         raise ValueError("cu_q must be contiguous int32 [S + 1]")
     if max_q_len < 0:
         raise ValueError(f"max_q_len={max_q_len} is negative")
-    device = _one_device(logits, tokens, parents, cu_q)
     s, row_stride = cu_q.shape[0] - 1, max(logits.stride(0), vocab) if n <= 1 else logits.stride(0)
     if row_stride < vocab:
         raise ValueError("the rows of logits overlap")
+    device = _one_device(logits, tokens, parents, cu_q)
     target, following = torch.empty_like(tokens), tokens.new_empty(s)
     path, counts = cu_q.new_empty(s, max_q_len), cu_q.new_empty(s)
     if n or s:
