@@ -465,11 +465,12 @@ int mip_paged_tree(void* out, int64_t out_stride_tok, int64_t out_stride_head, c
  *     positions[r]    = c + depth of node i (a root has depth 0)
  *     slot_mapping[r] = pool slot of cache index c + i, -1 past the table
  *     mask[r]         = the nodes on the path from i to its root, i among them, mask_words words a row
+ * and 0, -1 and no bits for rows of no node (those of n_rows outside the trees, nodes from max_q_len on).
  * max_q_len at most MIP_TREE_MAX_NODES (MIP_EUNSUPPORTED).
  */
 #define MIP_TREE_MAX_NODES 1024
 int mip_tree_index(int64_t* positions, int64_t* slot_mapping, uint64_t* mask, int32_t mask_words,
-                   const int32_t* parents, const int32_t* cu_q, const int32_t* ctx_start, const int32_t* block_tables,
+                   const int32_t* parents, int32_t n_rows, const int32_t* cu_q, const int32_t* ctx_start, const int32_t* block_tables,
                    int64_t bt_stride, int32_t num_seqs, int32_t max_q_len, int32_t block_size,
                    int32_t max_blocks_per_seq, void* stream);
 

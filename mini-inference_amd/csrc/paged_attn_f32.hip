@@ -294,7 +294,7 @@ __device__ __forceinline__ void attn_f32(const DecodeArgs& a, const TreeMask& tm
       // (A NaN among a tree row's scores has to stay one.)
       out[(q0 + tok) * a.out_sb + head * a.out_sh + d] = (TREE ? Ls != 0.f : Ls > 0.f) ? A / Ls : 0.f;
     } else {
-      const int64_t slot = (static_cast<int64_t>(TREE ? q0 + tok : q0) * a.hq + head) * a.nparts + part;
+      const int64_t slot = (static_cast<int64_t>(TREE ? trow * a.max_q_len + tok : q0) * a.hq + head) * a.nparts + part;
       a.ws_acc[slot * D + d] = A;
       if (d == 0) {
         a.ws_ml[slot * 2] = mx;

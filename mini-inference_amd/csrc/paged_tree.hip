@@ -50,7 +50,7 @@ typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint4 u4(const u32x4_t& x) { return __builtin_bit_cast(uint4, x); }
 
-constexpr int kMaxSeqs = 1024;  // sequences whose places fit in LDS
+constexpr int kMaxSeqs = 1024;  // sequences whose places fit in LDS; larger batches take several launches
 
 struct TreeArgs {
   char* out;
@@ -149,6 +149,7 @@ struct Shared {
   int start[kMaxSeqs];  // first step of every sequence's segments
   int cu[kMaxSeqs + 1], ctx[kMaxSeqs];
   uint32_t ok[2];       // byte w: every key that wavefront w copied exists and lies in a block of the pool
+  uint32_t redo;        // byte w: wavefront w found sums that need V as it is
 };
 
 // Node of query row r (group 1 has no 32-bit reciprocal).
@@ -221,6 +222,42 @@ struct Rows {
     // On the bits: the compiler takes a maximum of absolute values for a number and compares it as one.
     return __all(__float_as_uint(big) < 0x7f800000u);
   }
+  // Of the whole wavefront: whether in some dim every row's weighted mean is below 2^-16, where the rounding of V to
+  // fp16's subnormal grid (2^-25) would show beside the rounding of the output. First within each lane's rows, which
+  // settles nearly every piece; then over the lanes.
+  __device__ __forceinline__ bool tiny() const {
+    constexpr float kSmall = 0x1p-16f;
+    f32x4_t top[MT];
+    bool some = false;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const float inv = l[c][0] == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(l[c][0]);
+      some = some || l[c][0] != 0.0f;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = fabsf(acc[c][mt][i] * inv);
+          top[mt][i] = c ? fmax2(top[mt][i], x) : x;
+        }
+    }
+    auto least = [&] {
+      float low = INFINITY;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) low = top[mt][i] < low ? top[mt][i] : low;
+      return low;
+    };
+    if (!__any(some && least() < kSmall)) return false;
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1)
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top[mt][i] = fmax2(top[mt][i], __shfl_xor(top[mt][i], o));
+    return __any(least() < kSmall);
+  }
 };
 
 __device__ __forceinline__ uint32_t mask_window(const TreeArgs& a, const Piece& p, int tok, int key0) {
@@ -280,9 +317,12 @@ __device__ __forceinline__ void score_tile(const TreeArgs& a, const Piece& p, Ro
 }
 
 // The weights of block c from its scores: exp2(-inf - m) = 0 for a finite m; m stays -inf only while every score of the
-// row is -inf, and then 0 stands for it.
+// row is -inf, and then 0 stands for it. All weights carry a factor of 2^kLift: with it they reach 2^(kLift +
+// kRescaleLog2) = 2^15, within fp16, and the smallest that fp16 holds is 2^-31 of a row's largest, so that what a
+// long tail of small weights loses stays below the output's rounding (2^-32 each).
+constexpr float kLift = 7.0f;
 __device__ __forceinline__ void weights(const float (&sv)[8], float m, float scale_log2, float (&pr)[8]) {
-  const float nm = m == -INFINITY ? 0.0f : -m;
+  const float nm = m == -INFINITY ? 0.0f : kLift - m;
 #pragma unroll
   for (int i = 0; i < 8; ++i) pr[i] = fast_exp2(fmaf(sv[i], scale_log2, nm));
 }
@@ -549,9 +589,9 @@ __device__ __forceinline__ void private_pass(const TreeArgs& a, const Piece& p, 
 }
 
 // A workgroup's keys of a piece, staged by all its threads for all its wavefronts: two LDS stages of a step, the
-// next step's rows in registers meanwhile. WR x WK wavefronts: WK take different 32 keys of a step. bf16 V is staged
-// as fp16, once for all rows.
-template <int DT, int D, int WR, int WK, int NCK, int NC>
+// next step's rows in registers meanwhile. WR x WK wavefronts: WK take different 32 keys of a step. VT: the type in
+// which V is staged, fp16 (once for all rows) or its own.
+template <int DT, int VT, int D, int WR, int WK, int NCK, int NC>
 __device__ __forceinline__ void shared_pass(const TreeArgs& a, const Piece& p, Rows<D, NC>& rows, char* smem, Shared& sh,
                                             int w, int lane) {
   using P = Shape<D, WR, WK, NCK>;
@@ -591,7 +631,7 @@ __device__ __forceinline__ void shared_pass(const TreeArgs& a, const Piece& p, R
     for (int j = 0; j < NLD; ++j) {
       const int idx = tid + j * P::T, r = idx / CPR, c = idx % CPR;
       u32x4_t vv = vbuf[j];
-      if constexpr (DT == MIP_BF16) vv = bf16x8_to_f16x8(vv);
+      if constexpr (DT != VT) vv = bf16x8_to_f16x8(vv);
       *reinterpret_cast<u32x4_t*>(st + r * RB + ((c ^ (r & (CPR - 1))) * 16)) = kbuf[j];
       *reinterpret_cast<u32x4_t*>(st + P::TILE + r * RB + ((c ^ vsw<D>(r)) * 16)) = vv;
     }
@@ -638,7 +678,7 @@ __device__ __forceinline__ void shared_pass(const TreeArgs& a, const Piece& p, R
       }
       float sv[NC][8];
       score_tile<DT, D, NC>(a, p, rows, k, key0, real, grp, sv);
-      value_tile<MIP_F16, D, NC>(rows, vt, sv, a.scale_log2);
+      value_tile<VT, D, NC>(rows, vt, sv, a.scale_log2);
     }
     if (t + 1 < p.step1) stash(stage ^ 1);
     __syncthreads();
@@ -688,10 +728,18 @@ __device__ __forceinline__ void run_piece(const TreeArgs& a, const Piece& p, flo
   Rows<D, NC> rows;
   const int first = p.rb * (P::R / 16) + wr;
   rows.load(a, p, first, WR, i16, grp);
-  if constexpr (P::kPrivate)
+  if constexpr (P::kPrivate) {
     private_pass<DT, D, NC>(a, p, rows, (lchar_t*)(smem + w * P::kRing), wk, lane);
-  else
-    shared_pass<DT, D, WR, WK, NCK, NC>(a, p, rows, smem, sh, w, lane);
+  } else {
+    shared_pass<DT, MIP_F16, D, WR, WK, NCK, NC>(a, p, rows, smem, sh, w, lane);
+    if constexpr (DT == MIP_BF16) {  // the workgroup's keys again where they are too small for fp16
+      const bool redo = rows.tiny();
+      if (lane == 0) reinterpret_cast<uint8_t*>(&sh.redo)[w] = redo ? 1 : 0;
+      __syncthreads();
+      if (__builtin_amdgcn_readfirstlane(sh.redo) != 0)
+        shared_pass<DT, DT, D, WR, WK, NCK, NC>(a, p, rows, smem, sh, w, lane);
+    }
+  }
   // A wavefront whose accumulators hold inf or NaN does its part again.
   if (!rows.finite()) careful_pass<DT, D, NC, P::KT>(a, p, rows, first, WR, wk, lane);
   if constexpr (WK == 1) {
@@ -924,7 +972,7 @@ __global__ __launch_bounds__(256) void paged_tree_merge(TreeArgs a, int segs_per
 // over its LPR lanes alone); the states meet at the end. A key that the row does not see contributes
 // nothing at all, whatever its bytes are.
 // Long contexts of few rows are cut into parts of `tokens` keys (blockIdx.z), which leave their states in
-// ml [row][head][part][2] and acc [row][head][part][D].
+// ml [x][head][part][2] and acc [x][head][part][D], x = s * max_q_len + i of node i of sequence s.
 struct PartArgs {
   int hq, tokens, parts;
   float* ml;
@@ -1029,7 +1077,7 @@ __global__ __launch_bounds__(256) void paged_tree_row_kernel(TreeArgs a, PartArg
       reinterpret_cast<S*>(a.out)[r * a.out_st + static_cast<int64_t>(h) * a.out_sh + d] =
           from_f32<DT>(Ls == 0.0f ? 0.0f : A / Ls);
     } else {
-      const int64_t slot = (r * pt.hq + h) * pt.parts + part;
+      const int64_t slot = (x * pt.hq + h) * pt.parts + part;
       pt.acc[slot * D + d] = A;
       if (d == 0) {
         pt.ml[2 * slot] = top;
@@ -1048,7 +1096,7 @@ __global__ __launch_bounds__(kWave) void paged_tree_parts_kernel(TreeArgs a, Par
   const Seq p = seq_of(a, s);
   const int h = blockIdx.y, np = (keys_of(a, p) + pt.tokens - 1) / pt.tokens;
   if (i >= p.n || np < 2) return;
-  const int64_t r = static_cast<int64_t>(p.q0) + i, slot = (r * pt.hq + h) * pt.parts;
+  const int64_t r = static_cast<int64_t>(p.q0) + i, slot = (x * pt.hq + h) * pt.parts;
   float m = -INFINITY;
   for (int k = 0; k < np; ++k) m = fmax2(m, pt.ml[2 * (slot + k)]);
   for (int d = threadIdx.x; d < dim; d += kWave) {
@@ -1100,10 +1148,7 @@ Config pick(int d, int64_t rows) {
   return config_of<DT, 128, 4, 1, 2, 2>();
 }
 
-#ifndef K_BYP
-#define K_BYP 512
-#endif
-constexpr unsigned kMergeByPiece = K_BYP;
+constexpr unsigned kMergeByPiece = 512;  // column blocks up to which pieces are combined by piece
 constexpr int kMinShareKeys = 64;  // fewest keys a worker takes
 
 int compute_units() {
@@ -1124,7 +1169,7 @@ Plan plan_of(int num_seqs, int max_q_len, int hq, int hkv, int d, int bs, int ma
   Plan p;
   const int group = hq / hkv;
   const int64_t rows = static_cast<int64_t>(max_q_len) * group, cap = static_cast<int64_t>(max_blocks) * bs;
-  if ((dtype != MIP_F16 && dtype != MIP_BF16) || (d != 64 && d != 128) || num_seqs > kMaxSeqs) return p;
+  if ((dtype != MIP_F16 && dtype != MIP_BF16) || (d != 64 && d != 128)) return p;
   p.cfg = dtype == MIP_F16 ? pick<MIP_F16>(d, rows) : pick<MIP_BF16>(d, rows);
   const int64_t segs = hkv * ((rows + p.cfg.rows - 1) / p.cfg.rows), steps = (cap + p.cfg.keys - 1) / p.cfg.keys;
   if ((rows + 256) * group >= (int64_t{1} << 31) || segs * steps >= (int64_t{1} << 30) || segs * num_seqs * steps >= (int64_t{1} << 30) ||
@@ -1215,6 +1260,13 @@ extern "C" size_t mip_paged_tree_workspace(int32_t num_seqs, int32_t max_q_len, 
       head_dim <= 0 || block_size <= 0 || max_blocks_per_seq <= 0 ||
       static_cast<int64_t>(max_blocks_per_seq) * block_size >= (int64_t{1} << 30))
     return 0;
+  if (num_seqs > tree::kMaxSeqs) {  // several launches, one after the other
+    const size_t full = mip_paged_tree_workspace(tree::kMaxSeqs, max_q_len, num_heads, num_kv_heads, head_dim, block_size,
+                                                 max_blocks_per_seq, dtype);
+    const size_t rest = mip_paged_tree_workspace(num_seqs % tree::kMaxSeqs, max_q_len, num_heads, num_kv_heads, head_dim,
+                                                 block_size, max_blocks_per_seq, dtype);
+    return full > rest ? full : rest;
+  }
   const int64_t cap = static_cast<int64_t>(max_blocks_per_seq) * block_size;
   // The larger of what the kernels need that may take the call (its alignment is not known here).
   const int64_t main =
@@ -1250,6 +1302,21 @@ extern "C" int mip_paged_tree(void* out, int64_t out_stride_tok, int64_t out_str
                             static_cast<uint64_t>(out_stride_head * es);
   if (((q_bits | out_bits) & (es - 1)) || ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15))
     return MIP_EINVAL;
+  if (num_seqs > tree::kMaxSeqs) {
+    const size_t need = mip_paged_tree_workspace(num_seqs, max_q_len, num_heads, num_kv_heads, head_dim, block_size,
+                                                 max_blocks_per_seq, dtype);
+    if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255)))
+      return MIP_EINVAL;
+    for (int32_t s0 = 0; s0 < num_seqs; s0 += tree::kMaxSeqs) {
+      const int32_t some = num_seqs - s0 < tree::kMaxSeqs ? num_seqs - s0 : tree::kMaxSeqs;
+      const int rc = mip_paged_tree(out, out_stride_tok, out_stride_head, q, q_stride_tok, q_stride_head, k_cache, v_cache,
+                                    num_cache_blocks, block_tables + s0 * bt_stride, bt_stride, cu_q + s0, ctx_start + s0,
+                                    mask, mask_stride, mask_words, some, max_q_len, num_heads, num_kv_heads, head_dim,
+                                    block_size, max_blocks_per_seq, scale, workspace, workspace_bytes, dtype, stream);
+      if (rc != MIP_OK) return rc;
+    }
+    return MIP_OK;
+  }
 
   tree::TreeArgs a{};
   a.out = static_cast<char*>(out);

@@ -167,7 +167,7 @@ _SIGNATURES = {
          _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _vp, _sz, _i32, _vp],
     ),
     "mip_paged_tree_workspace": (_sz, [_i32] * 8),
-    "mip_tree_index": (_c.c_int, [_vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp]),
+    "mip_tree_index": (_c.c_int, [_vp, _vp, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp]),
     "mip_tree_verify": (
         _c.c_int,
         [_vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _i32, _i32, _vp, _sz, _i32, _vp],

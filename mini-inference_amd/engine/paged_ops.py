@@ -776,17 +776,23 @@ def _tree_rows(cu_q: torch.Tensor, block_tables: torch.Tensor, ctx_start: torch.
     return s, mb
 
 
-def _scratch(workspace: torch.Tensor | None, device: torch.device, need: int) -> tuple[int | None, int]:
-    """Address and size of a call's scratch memory: the caller's, or the device's shared buffer."""
+def _scratch(workspace: torch.Tensor | None, device: torch.device, need: int) -> torch.Tensor | None:
+    """A call's scratch memory: the caller's, or new memory from the current stream's allocator.
+
+    The latter is the call's own: calls on several streams and captured graphs (whose private pool it comes from) do
+    not meet in it, and the allocator hands it on only behind the call's kernels on its stream."""
     if workspace is None:
-        workspace = _workspace.get(device, need)
-    elif need and workspace.numel() * workspace.element_size() < need:
+        return torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    if need and workspace.numel() * workspace.element_size() < need:
         raise ValueError(f"workspace holds {workspace.numel() * workspace.element_size()} bytes, needs {need}")
-    elif workspace.device != device or not workspace.is_contiguous():
+    if workspace.device != device or not workspace.is_contiguous():
         raise ValueError("workspace must be a contiguous tensor on the call's device")
-    if workspace is None:
-        return None, 0
-    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    return workspace
+
+
+def _extent(workspace: torch.Tensor | None) -> tuple[int | None, int]:
+    """Address and size of scratch memory."""
+    return (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
 
 
 @lru_cache(4096)
@@ -810,8 +816,8 @@ def tree_index(parents: torch.Tensor, cu_q: torch.Tensor, ctx_start: torch.Tenso
     root). ``positions`` (int64 ``[N]``) are ``ctx_start[s]`` + depth; ``slot_mapping`` (int64 ``[N]``) the
     pool slots of cache indexes ``ctx_start[s] + i`` (-1 past the table); ``mask`` (int64 ``[N, W]``,
     ``W = ceil(max_q_len / 64)``) has bit ``j % 64`` of word ``j // 64`` set for the nodes j on the path to the
-    root, the node itself among them: what :func:`paged_tree` takes. Trees of up to 1024 nodes. Rows of
-    no sequence are not written.
+    root, the node itself among them: what :func:`paged_tree` takes. Trees of up to 1024 nodes. Rows of no node (a
+    padded batch's, and a tree's from ``max_q_len`` on) have position 0, slot -1 and no bits.
     """
     s, mb = _tree_rows(cu_q, block_tables, ctx_start, max_q_len, max_blocks)
     if parents.dtype != torch.int32 or parents.dim() != 1 or not parents.is_contiguous():
@@ -820,9 +826,9 @@ def tree_index(parents: torch.Tensor, cu_q: torch.Tensor, ctx_start: torch.Tenso
     n, words = parents.shape[0], (max_q_len + 63) // 64
     positions = torch.empty(n, dtype=torch.int64, device=device)
     slots, mask = torch.empty_like(positions), positions.new_empty(n, words)
-    if n and s and max_q_len:
+    if n:
         _call_on(device, _native.load().mip_tree_index,
-                 (positions.data_ptr(), slots.data_ptr(), mask.data_ptr(), words, parents.data_ptr(), cu_q.data_ptr(),
+                 (positions.data_ptr(), slots.data_ptr(), mask.data_ptr(), words, parents.data_ptr(), n, cu_q.data_ptr(),
                   ctx_start.data_ptr(), block_tables.data_ptr(), block_tables.stride(0), s, max_q_len, block_size, mb),
                  "mip_tree_index")
     return positions, slots, mask
@@ -860,14 +866,12 @@ def _tree_args(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
     if not (n and s and max_q_len):
         return None, out, None
     code = dtype_code(q.dtype)
-    need = _tree_bytes(device, s, max_q_len, hq, hkv, d, bs, mb, code)
-    if workspace is None:
-        workspace = _workspace.get(device, need)
-    ws_ptr, ws_bytes = _scratch(workspace, device, need)
+    workspace = _scratch(workspace, device, _tree_bytes(device, s, max_q_len, hq, hkv, d, bs, mb, code))
+    ws_ptr, ws_bytes = _extent(workspace)
     return (out.data_ptr(), out.stride(0), out.stride(1), q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
             v_cache.data_ptr(), nb, block_tables.data_ptr(), block_tables.stride(0), cu_q.data_ptr(),
-            ctx_start.data_ptr(), mask.data_ptr(), mask.stride(0), mask.shape[1], s, max_q_len, hq, hkv, d, bs, mb,
-            scale, ws_ptr, ws_bytes, code), out, workspace
+            ctx_start.data_ptr(), mask.data_ptr(), max(mask.stride(0), mask.shape[1]) if n == 1 else mask.stride(0),
+            mask.shape[1], s, max_q_len, hq, hkv, d, bs, mb, scale, ws_ptr, ws_bytes, code), out, workspace
 
 
 def paged_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -885,11 +889,12 @@ def paged_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
 
     16-bit types at head_dim 64 / 128 run on the matrix cores, long contexts of few rows cut into pieces and
     combined; fp32 at those head sizes on the fp32 matrix cores; other head sizes (powers of two from 8 to 256) and short
-    calls one query row at a time. Scratch memory is shared by the calls of a device, which must then be ordered; pass
-    ``workspace`` (:func:`tree_workspace_bytes`) to calls that may run at once.
+    calls one query row at a time. Scratch memory is allocated for the call on the current stream, unless ``workspace``
+    (:func:`tree_workspace_bytes`) is given, which calls that may run at once must not share. ``out`` must not overlap
+    the inputs.
     """
-    args, out, _ = _tree_args(q, k_cache, v_cache, block_tables, cu_q, ctx_start, mask, max_q_len, scale, out, max_blocks,
-                              workspace)
+    args, out, workspace = _tree_args(q, k_cache, v_cache, block_tables, cu_q, ctx_start, mask, max_q_len, scale, out,
+                                      max_blocks, workspace)
     if args is not None:
         _call_on(q.device, _native.load().mip_paged_tree, args, "mip_paged_tree")
     return out
@@ -968,7 +973,8 @@ def tree_verify(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
     path, counts = cu_q.new_empty(s, max_q_len), cu_q.new_empty(s)
     if n or s:
         lib = _native.load()
-        ws_ptr, ws_bytes = _scratch(workspace, device, _verify_bytes(n, vocab, code))
+        workspace = _scratch(workspace, device, _verify_bytes(n, vocab, code))
+        ws_ptr, ws_bytes = _extent(workspace)
         _call_on(device, lib.mip_tree_verify,
                  (target.data_ptr(), path.data_ptr(), counts.data_ptr(), following.data_ptr(), logits.data_ptr(),
                   row_stride, n, vocab, tokens.data_ptr(), parents.data_ptr(), cu_q.data_ptr(), s, max_q_len, ws_ptr,
@@ -984,6 +990,8 @@ def tree_commit(k_pool: torch.Tensor, v_pool: torch.Tensor, block_tables: torch.
     ``counts`` (int32 ``[S]``) as :func:`tree_verify` returns them: the row of cache index ``ctx_start[s] + path[s, d]``
     moves to ``ctx_start[s] + d`` for ``d < counts[s]``, as if all were read before any is written. A path rises and
     has ``path[s, d] >= d``; an entry that breaks this, or whose place lies outside the table or the pool, ends it.
+    No two sequences may own the blocks that rows move in (a block that a fork shares is copied before the nodes are
+    appended: ``PagedKVCache.prepare_writes``).
     """
     if k_pool.dim() != 5 or k_pool.shape != v_pool.shape or not (k_pool.is_contiguous() and v_pool.is_contiguous()):
         raise ValueError("k_pool/v_pool must be contiguous [L, num_blocks, Hkv, block_size, D] tensors of one shape")

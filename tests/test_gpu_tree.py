@@ -185,6 +185,68 @@ def test_large_values(gpu, dtype, nodes):
     step.check(run(gpu, step))
 
 
+@pytest.mark.parametrize("dtype,d,hq,hkv,nodes", [
+    ("bfloat16", 64, 14, 2, [3, 12]), ("bfloat16", 64, 14, 2, [40, 5]), ("bfloat16", 128, 28, 4, [12]), ("bfloat16", 64, 14, 2, [2]),
+    ("float32", 64, 14, 2, [12]), ("bfloat16", 32, 14, 2, [12])])
+@pytest.mark.parametrize("where", ["all", "one dim", "one sequence"])
+def test_values_below_fp16(gpu, dtype, d, hq, hkv, nodes, where):
+    """Values of about 2^-30, everywhere or beside ordinary ones, keep their relative accuracy."""
+    announce(f"paged_tree small values {dtype} d={d} nodes={nodes} {where}")
+    step = Step(dtype, d, hq, hkv, 16, [300] * len(nodes), nodes, seed=15)
+    if where == "all":
+        step.v *= 2.0**-30
+    elif where == "one dim":
+        step.v[..., 7] *= 2.0**-30
+    else:
+        step.v[torch.tensor(step.tables[0])] *= 2.0**-30
+    got = run(gpu, step).double().cpu().numpy()
+    out, spread, reach = step.want()
+    half_step = torch.finfo(DTYPES[dtype]).eps / 2
+    delta = (d + 2) * 2.0**-24 * reach + 2.0**-21 + 400 * 2.0**-23 + (0 if dtype == "float32" else 2.0**-11)
+    small = np.zeros(out.shape, bool)
+    if where == "all":
+        small[:] = True
+    elif where == "one dim":
+        small[..., 7] = True
+    else:
+        small[:nodes[0]] = True
+    bound = half_step * 1.01 * np.abs(out) + 2.05 * delta[..., None] * spread + 400 * 2.0**-31 * spread
+    assert (np.abs(got - out) <= bound)[small].all()
+    step.check(torch.from_numpy(got))
+
+
+def test_a_long_tail_of_small_weights(gpu):
+    """One key far above 30000 others whose weights (2^-25.5 of its own) fp16 alone would round by half: each is held to
+    2^-32 of the largest."""
+    announce("paged_tree tail of small weights")
+    step = Step("float16", 64, 2, 1, 16, [30000], [40], seed=16, scale=1.0)
+    step.qkv.zero_()
+    step.k.zero_()
+    step.qkv[:, 0] = step.qkv[:, 64] = 1.0
+    step.k[step.tables[0][3], 0, 5, 0] = 25.5 * math.log(2.0)
+    step.v.fill_(1.0)
+    step.v[step.tables[0][3], 0, 5] = 0.0
+    out, _, _ = step.want()
+    got = run(gpu, step).double().cpu().numpy()
+    assert 5e-4 < out.min() and np.abs(got - out).max() <= 30040 * 2.0**-32 + 2.0**-11 * out.max() * 3
+
+
+@pytest.mark.parametrize("dtype,d,start", [("float16", 64, 600), ("float16", 64, 20), ("float32", 64, 900), ("float32", 32, 900),
+                                           ("bfloat16", 128, 600), ("float32", 64, 20)])
+def test_trees_longer_than_max_q_len_end_there(gpu, dtype, d, start):
+    """Nodes from max_q_len on are no rows and no keys; their output rows stay as they were."""
+    announce(f"paged_tree clipped trees {dtype} d={d} start={start}")
+    step = Step(dtype, d, 4, 2, 16, [start, 8, start], [10, 3, 7], seed=17, kind="free")
+    args = step.to(gpu)
+    out = torch.full((20, 4, d), 7.0, dtype=DTYPES[dtype], device=gpu)
+    run(gpu, step, max_q_len=4, out=out)
+    assert (out[4:10] == 7).all() and (out[17:] == 7).all()
+    keep = [0, 1, 2, 3, 10, 11, 12, 13, 14, 15, 16]
+    step.nodes, step.mask, step.qkv = [4, 3, 4], step.mask[keep], step.qkv[keep]
+    step.check(out[keep])
+    del args
+
+
 @pytest.mark.parametrize("dtype,d", [("float16", 64), ("bfloat16", 128), ("float32", 64), ("float16", 32)])
 def test_rows_that_see_nothing_and_rows_of_nobody(gpu, dtype, d):
     announce(f"paged_tree empty rows {dtype} d={d}")
@@ -450,6 +512,66 @@ def test_two_streams_with_their_own_scratch(gpu):
     torch.cuda.synchronize()
     for i, out in enumerate(got):
         assert torch.equal(out, want[i % 2])
+
+
+def test_calls_on_two_streams_and_two_graphs_do_not_meet(gpu):
+    """Without ``workspace`` every call has scratch memory of its own: calls in flight on two streams, and two captured
+    graphs replayed on two streams, give what each gives alone."""
+    from engine import paged_ops
+
+    announce("paged_tree and tree_verify on two streams, eager and captured")
+    args = [Step("bfloat16", 64, 14, 2, 16, [4000, 50], [5, 12], seed=s).to(gpu) for s in (1, 2)]
+    logits = [torch.randn(17, 50000, device=gpu) for _ in args]
+    tokens, parents = torch.zeros(17, dtype=torch.int64, device=gpu), torch.zeros(17, dtype=torch.int32, device=gpu)
+
+    def work(i):
+        return (paged_ops.paged_tree(**args[i]), *paged_ops.tree_verify(logits[i], tokens, parents, args[i]["cu_q"], 12))
+
+    want = [work(i) for i in (0, 1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in args]
+    got = []
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append((i, work(i)))
+    torch.cuda.synchronize()
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in args], []
+    for i, g in enumerate(graphs):
+        with torch.cuda.graph(g):
+            outs.append(work(i))
+    for _ in range(5):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        got += [(i, [x.clone() for x in o]) for i, o in enumerate(outs)]
+        torch.cuda.synchronize()
+    for i, out in got:
+        assert all(torch.equal(x, y) for x, y in zip(out, want[i]))
+
+
+def test_index_of_a_padded_batch(gpu):
+    """Rows of no node (ahead of the first tree, behind the last, past max_q_len) get slot -1 and no bits."""
+    from engine import paged_ops
+
+    announce("tree_index padded")
+    i32 = dict(dtype=torch.int32, device=gpu)
+    for most, sizes in ((3, [5, 2]), (70, [90, 3])):
+        n = 2 + sum(sizes) + 4
+        parents = torch.tensor([9, 9] + [p for k in sizes for p in range(-1, k - 1)] + [9] * 4, **i32)
+        cu = torch.tensor([2, 2 + sizes[0], 2 + sum(sizes)], **i32)
+        tables = torch.tensor([[4] * 8, [6] * 8], **i32)
+        pos, slots, mask = paged_ops.tree_index(parents, cu, torch.tensor([10, 3], **i32), tables, most, 16)
+        live = [2 + i for i in range(most)] + [2 + sizes[0] + i for i in range(sizes[1])]
+        want = ref.index([range(-1, most - 1), range(-1, sizes[1] - 1)], [10, 3], [[4] * 8, [6] * 8], 16, 8, mask.shape[1])
+        for got, full, blank in zip((pos, slots, mask), want, (0, -1, 0)):
+            got = got.cpu().numpy()
+            assert np.array_equal(got[live], full)
+            assert (np.delete(got, live, axis=0) == blank).all()
+    pos, slots, mask = paged_ops.tree_index(torch.zeros(3, **i32), torch.zeros(1, **i32), torch.zeros(0, **i32),
+                                            torch.zeros(0, 1, **i32), 0, 16)
+    assert pos.tolist() == [0] * 3 and slots.tolist() == [-1] * 3 and mask.shape == (3, 0)
 
 
 def test_a_captured_step_replays_on_new_inputs(gpu):

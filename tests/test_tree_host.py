@@ -141,14 +141,18 @@ def test_c_entries_check_before_they_launch():
     assert attend(d=96) == no and attend(d=512) == no
     size = lib.mip_paged_tree_workspace
     assert size(8, 3, 4, 2, 64, 16, 1024, _native.MIP_F16) > 0
+    large = size(1024, 3, 4, 2, 64, 16, 1024, _native.MIP_F16)
+    assert large > 0 and size(5000, 3, 4, 2, 64, 16, 1024, _native.MIP_F16) == large
+    assert attend(mb=1024, bt_stride=1024, s=5000, ws=p, ws_bytes=large - 1) == bad
     assert size(0, 3, 4, 2, 64, 16, 1024, _native.MIP_F16) == 0 and size(1, 3, 3, 2, 64, 16, 4, _native.MIP_F16) == 0
 
-    def index(words=1, s=1, m=3, bs=16, mb=4, parents=p):
-        return lib.mip_tree_index(p, p, p, words, parents, p, p, p, 4, s, m, bs, mb, None)
+    def index(words=1, n=3, s=1, m=3, bs=16, mb=4, parents=p, tables=p):
+        return lib.mip_tree_index(p, p, p, words, parents, n, p, p, tables, 4, s, m, bs, mb, None)
 
-    assert index(s=0) == ok and index(m=0) == ok
-    assert index(m=1025) == no
-    for kw in (dict(words=0), dict(words=17), dict(s=-1), dict(bs=3), dict(mb=5), dict(mb=0), dict(parents=None), dict(m=65)):
+    assert index(n=0) == ok
+    assert index(m=1025) == no and index(s=1 << 24) == no
+    for kw in (dict(words=0), dict(words=17), dict(s=-1), dict(n=-1), dict(bs=3), dict(mb=5), dict(mb=0), dict(parents=None),
+               dict(tables=None), dict(m=65)):
         assert index(**kw) == bad, kw
 
     def verify(n=3, vocab=100, stride=100, s=1, m=3, ws=p, ws_bytes=1 << 20, dt=_native.MIP_F32, logits=p):
