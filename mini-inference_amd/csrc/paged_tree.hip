@@ -231,8 +231,9 @@ struct Rows {
     bool some = false;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const float inv = l[c][0] == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(l[c][0]);
-      some = some || l[c][0] != 0.0f;
+      const bool counts = live[c] && l[c][0] != 0.0f;
+      const float inv = counts ? __builtin_amdgcn_rcpf(l[c][0]) : 0.0f;
+      some = some || counts;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -249,7 +250,7 @@ struct Rows {
         for (int i = 0; i < 4; ++i) low = top[mt][i] < low ? top[mt][i] : low;
       return low;
     };
-    if (!__any(some && least() < kSmall)) return false;
+    if (!__any(some && least() < kSmall)) return false;  // (a NaN is not small)
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1)
 #pragma unroll
@@ -736,8 +737,18 @@ __device__ __forceinline__ void run_piece(const TreeArgs& a, const Piece& p, flo
       const bool redo = rows.tiny();
       if (lane == 0) reinterpret_cast<uint8_t*>(&sh.redo)[w] = redo ? 1 : 0;
       __syncthreads();
-      if (__builtin_amdgcn_readfirstlane(sh.redo) != 0)
-        shared_pass<DT, DT, D, WR, WK, NCK, NC>(a, p, rows, smem, sh, w, lane);
+      if (__builtin_amdgcn_readfirstlane(sh.redo) != 0) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {  // one column block at a time: few registers beside the others' sums
+          Rows<D, 1> one;
+          one.load(a, p, first + c * WR, 0, i16, grp);
+          shared_pass<DT, DT, D, WR, WK, NCK, 1>(a, p, one, smem, sh, w, lane);
+          rows.m[c] = one.m[0];
+          rows.l[c] = one.l[0];
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) rows.acc[c][mt] = one.acc[0][mt];
+        }
+      }
     }
   }
   // A wavefront whose accumulators hold inf or NaN does its part again.
@@ -1132,19 +1143,26 @@ Config config_of() {
           paged_tree_merge<DT, D, P::R, true>, P::R, P::KT, OCC, P::kRec};
 }
 
-// The workgroup's shape by the most rows a sequence can have.
+// The workgroup's shape by the most rows a segment's kv head can have, and the products of the call (sequences x kv
+// heads x rows x keys). Wavefronts with the same 16, 32 or 64 rows and keys of their own need no staging together and
+// cut a segment finely; wavefronts with rows of their own that share keys read each key a quarter as often. The
+// second pays for more rows than 64 once the call is large (graph replay, us, own keys / shared; sequences x nodes of 7
+// rows; d64, 2 kv heads: 16 x 24 over 1024 keys 19.1/23.0, 64 x 48 over 256 21.9/29.1, 64 x 24 over 1024 (22M) 28.6/30.8,
+// 64 x 32 over 1024 (29M) 36.7/32.5, 64 x 48 over 1024 43.2/37.9, 64 x 64 over 4096 109/84.7; d128, 4 kv heads: 4 x 24
+// over 4096 28.7/32.6, 1 x 16 over 32768 (15M) 33.4/34.8, 16 x 48 over 1024 (22M) 49.2/41.5, 16 x 64 over 4096 137/83.4).
+// d64 with shared keys: 32 rows a wavefront and three workgroups a CU against 64 and two, 64 x 64 over 512 36.0/39.0,
+// 256 x 64 over 512 66.9/73.2, 64 x 64 over 4096 87.0/85.8.
 template <int DT>
-Config pick(int d, int64_t rows) {
+Config pick(int d, int64_t rows, int64_t products) {
   if (d == 64) {
     if (rows <= 16) return config_of<DT, 64, 1, 4, 1, 2>();
     if (rows <= 32) return config_of<DT, 64, 1, 4, 2, 2>();
-    if (rows <= 64) return config_of<DT, 64, 1, 4, 4, 2>();
-    if (rows <= 128) return config_of<DT, 64, 2, 2, 4, 2>();
-    return config_of<DT, 64, 4, 1, 4, 2>();
+    if (rows <= 64 || products <= 28 << 20) return config_of<DT, 64, 1, 4, 4, 2>();
+    return config_of<DT, 64, 4, 1, 2, 3>();
   }
   if (rows <= 16) return config_of<DT, 128, 1, 4, 1, 1>();
   if (rows <= 32) return config_of<DT, 128, 1, 4, 2, 1>();
-  if (rows <= 64) return config_of<DT, 128, 1, 4, 4, 1>();
+  if (rows <= 64 || products <= 16 << 20) return config_of<DT, 128, 1, 4, 4, 1>();
   return config_of<DT, 128, 4, 1, 2, 2>();
 }
 
@@ -1170,7 +1188,8 @@ Plan plan_of(int num_seqs, int max_q_len, int hq, int hkv, int d, int bs, int ma
   const int group = hq / hkv;
   const int64_t rows = static_cast<int64_t>(max_q_len) * group, cap = static_cast<int64_t>(max_blocks) * bs;
   if ((dtype != MIP_F16 && dtype != MIP_BF16) || (d != 64 && d != 128)) return p;
-  p.cfg = dtype == MIP_F16 ? pick<MIP_F16>(d, rows) : pick<MIP_BF16>(d, rows);
+  const int64_t products = static_cast<int64_t>(num_seqs) * hkv * rows * cap;
+  p.cfg = dtype == MIP_F16 ? pick<MIP_F16>(d, rows, products) : pick<MIP_BF16>(d, rows, products);
   const int64_t segs = hkv * ((rows + p.cfg.rows - 1) / p.cfg.rows), steps = (cap + p.cfg.keys - 1) / p.cfg.keys;
   if ((rows + 256) * group >= (int64_t{1} << 31) || segs * steps >= (int64_t{1} << 30) || segs * num_seqs * steps >= (int64_t{1} << 30) ||
       segs * num_seqs >= (int64_t{1} << 24))
