@@ -904,13 +904,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
   }
 }
 
-// Combine the pieces of a split segment. Workgroup (x, cb, z): column block cb of segment x = (sequence, (kv head, row
-// block)). BY_PIECE: two dim tiles (z) of the block, each wavefront a quarter of the pieces (few segments, cut into many
-// pieces each: more workgroups and shorter chains); else all its dims, each wavefront a quarter of them.
+// Combine the pieces of a split segment x = (sequence, (kv head, row block)). BY_PIECE: workgroup (x, cb, z) takes two
+// dim tiles (z) of column block cb, each wavefront a quarter of the pieces (few segments, cut into many pieces each:
+// more workgroups and shorter chains). Else every wavefront of workgroup (x, y) a whole column block of its own, 4 y + w
+// (64 x 33-64 nodes of 7 rows, d64, 33 MB of records: 10.7 us, 13.8 with a quarter of a block's dims a wavefront).
 template <int DT, int D, int R, bool BY_PIECE>
 __global__ __launch_bounds__(256) void paged_tree_merge(TreeArgs a, int segs_per_seq, int keys_per_step) {
-  constexpr int MT = D / 16, PER = BY_PIECE ? 2 : MT / 4;
-  const int s = blockIdx.x / segs_per_seq, seg = blockIdx.x - s * segs_per_seq, cb = blockIdx.y;
+  constexpr int MT = D / 16, PER = BY_PIECE ? 2 : MT;
+  const int lane = threadIdx.x & (kWave - 1), i16 = lane & 15, w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int s = blockIdx.x / segs_per_seq, seg = blockIdx.x - s * segs_per_seq;
+  const int cb = BY_PIECE ? blockIdx.y : blockIdx.y * 4 + w;
   Piece p;
   p.s = s;
   p.q = seq_of(a, s);
@@ -926,8 +929,7 @@ __global__ __launch_bounds__(256) void paged_tree_merge(TreeArgs a, int segs_per
   p.kvh = seg / nrb;
   p.rb = seg - p.kvh * nrb;
   if (p.rb * R + cb * 16 >= p.q.n * a.group) return;
-  const int lane = threadIdx.x & (kWave - 1), i16 = lane & 15, w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int mt0 = BY_PIECE ? 2 * blockIdx.z : w * PER;
+  const int mt0 = BY_PIECE ? 2 * blockIdx.z : 0;
   constexpr int64_t kRec = 2 * R + static_cast<int64_t>(R) * D;
   // The segment's first piece ends inside it (record 1 of its worker); the others begin inside it (record 0).
   auto record = [&](int x) { return a.ws_rec + (static_cast<int64_t>(x) * 2 + (x == w0 ? 1 : 0)) * kRec; };
@@ -1387,7 +1389,7 @@ extern "C" int mip_paged_tree(void* out, int64_t out_stride_tok, int64_t out_str
         hipLaunchKernelGGL(p.cfg.merge_by_piece, dim3(segs, blocks, head_dim / 32), dim3(256), 0, s, a, p.segs_per_seq,
                            p.cfg.keys);
       else
-        hipLaunchKernelGGL(p.cfg.merge, dim3(segs, blocks), dim3(256), 0, s, a, p.segs_per_seq, p.cfg.keys);
+        hipLaunchKernelGGL(p.cfg.merge, dim3(segs, (blocks + 3) / 4), dim3(256), 0, s, a, p.segs_per_seq, p.cfg.keys);
     }
     return status_from_hip(hipGetLastError());
   }
