@@ -1,5 +1,6 @@
 // Paged attention in fp32 on the matrix cores (gfx950): decode partitions and packed prefill, at
-// head_dim 64 or 128 and up to 16 query heads per kv head.
+// head_dim 64 or 128 and up to 16 query heads per kv head; and drafted trees (paged_tree.hip), whose rows
+// see what their masks name, for any group.
 //
 // Reference semantics: engine/kv_cache.py:615-620 (decode) and :268-294 (packed prefill), fp32
 // throughout: v_mfma_f32_16x16x4_f32 multiplies and accumulates in fp32, the softmax is fp32.

@@ -15,26 +15,38 @@
 //
 // Work split. A sequence's query rows are its (node, head of the kv head's group) pairs, packed
 // node-major; a segment is (sequence, kv head, block of R rows) and has ceil((c + n) / KT) steps of KT
-// keys. Segments of very different lengths share the chip, and one long sequence has to fill it, so
-// segments of more than L steps are cut into pieces of at most L (about as many steps as a workgroup's
-// equal share); a piece leaves its rows' maxima, sums and unnormalised outputs in the workspace and a
-// second kernel combines them. L and each piece's place follow from cu_q and ctx_start on the device:
-// the grid depends on the integer arguments alone.
+// keys. Segments of very different lengths share the chip, and one long sequence has to fill it, so the
+// steps of all segments form one row and every workgroup takes an equal share of it; a cut that falls
+// close to a segment's end moves there. A piece that is not a whole segment leaves its rows' maxima, sums
+// and unnormalised outputs in a record (D + 2 floats a row) in the workspace, and a second kernel
+// combines them. The shares follow from cu_q and ctx_start on the device: the grid depends on the integer
+// arguments alone, so a captured call serves other lengths.
 //
-// A workgroup is WR x WK wavefronts: WR take different rows (NC blocks of 16 each) of the same keys, WK
-// take different 32 keys of a step for the same rows and meet at the piece's end. Few rows use WK = 4 (no
-// wavefront idles), many WR = 4 (each key staged once serves 256 rows). All threads copy the step's K and
-// V rows into LDS (two stages; the next step's rows travel in registers meanwhile); a wavefront then
-// computes
+// A wavefront computes, for NC blocks of 16 rows and 32 keys at a time,
 //   S^T[16 keys x 16 rows] = K . Q^T     v_mfma_f32_16x16x32, Q^T in registers
 //   O^T[D x 16 rows]      += V^T . P^T   v_mfma_f32_16x16x32 over 32 keys
-// with a base-2 online softmax. V^T comes from transposing LDS reads; P is in the layout of S^T.
+// with a base-2 online softmax whose maximum is raised only when a row's grows by more than 2^kRescaleLog2.
+// V^T comes from transposing LDS reads; P is in the layout of S^T. Two shapes of a workgroup:
+//   own keys     WR = 1, WK = 4: all wavefronts have the same rows and each 32 keys of a step of 128, which
+//                it fetches by itself: direct global -> LDS loads into two tiles of its own, no barrier in the
+//                loop. The four meet at the piece's end. For few rows, and for small calls.
+//   shared keys  WR = 4, WK = 1: each wavefront has rows of its own; all threads stage a step of 32 keys
+//                (two LDS stages, the next step's rows in registers meanwhile). For many rows.
+// (Direct loads for the shared shape were slower: 64 x 33-64 nodes of 7 rows 58 -> 66 us, one of 61 nodes over
+// 32000 keys 63 -> 104: four wavefronts wait at a barrier for loads that registers would have held back.)
 //
-// Roundings. Scores, sums and accumulators are fp32. The weights enter the V product as fp16 (2^-11
-// relative; the sums are taken of the rounded weights, so the error of a lone key cancels), bf16 V is
-// staged as fp16 (exact below 65536). A piece whose accumulators end up inf or NaN runs again with V
-// as it is, weights in two parts (their sum holds them to 2^-16 and better), and every inf or NaN of V
-// applied to the rows that see its key alone: a masked key must not reach a row as 0 * inf.
+// Roundings. Scores, sums and accumulators are fp32. fp16 V: the weights enter the product as fp16 (2^-11
+// relative; the sums are taken of the rounded weights, so the error of a lone key cancels). bf16 V with
+// own keys: V as it is, weights as a bf16 value and its remainder (2^-16); with shared keys V is staged
+// as fp16, once for all rows (exact from 2^-17 to 65280; one product instead of two: 65.1 -> 59.7 us and
+// 71.5 -> 63.5 on the two cases above), and a piece in which some dim's means are so small that this could
+// show runs again with V as it is. A wavefront whose accumulators end up inf or NaN does its part of a
+// piece again in a careful pass, which adds each value to the rows that see its key alone: a masked key
+// must not reach a row as 0 * inf.
+//
+// Measured (graph replay, us a call, both kernels): 128 sequences of 4-8 nodes, 28q/4kv d128, 512-8192
+// keys: 171, 725 MB at 4.2 TB/s; 64 x 33-64 nodes, 14q/2kv d64, 128-4096 keys: 51, 231 TFLOP/s; 61 nodes over
+// 32000 keys, 28q/4kv d128: 65, 430 TFLOP/s; 32 x 8-24 nodes, 128-1024 keys: 20; 5 nodes over 37 keys: 4.0.
 #include "paged_decode_common.h"
 
 namespace mip {
@@ -107,7 +119,6 @@ __device__ __forceinline__ u32x4_t bf16x8_to_f16x8(const u32x4_t& v) {
   };
   return u32x4_t{cv(v[0]), cv(v[1]), cv(v[2]), cv(v[3])};
 }
-
 
 template <int D, int WR, int WK, int NC>
 struct Shape {
@@ -984,6 +995,7 @@ __global__ __launch_bounds__(256) void paged_tree_merge(TreeArgs a, int segs_per
 // takes 64 / LPR keys at once and every key's row lanes keep a softmax state of their own (a score is summed
 // over its LPR lanes alone); the states meet at the end. A key that the row does not see contributes
 // nothing at all, whatever its bytes are.
+// Bound by latency at the sizes that it is for (5 nodes over 37 keys, 14 heads of 64: 4.0 us a call).
 // Long contexts of few rows are cut into parts of `tokens` keys (blockIdx.z), which leave their states in
 // ml [x][head][part][2] and acc [x][head][part][D], x = s * max_q_len + i of node i of sequence s.
 struct PartArgs {
