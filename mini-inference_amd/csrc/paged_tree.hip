@@ -612,29 +612,46 @@ __device__ __forceinline__ void shared_pass(const TreeArgs& a, const Piece& p, R
   const int32_t* table = a.bt + static_cast<int64_t>(p.s) * a.bt_stride;
   const int last = p.last;
   rows.clear();
+  // A wavefront's chunks of one copy are RW consecutive rows of one block (blocks have RW rows at least), 1 KB: block
+  // and address are scalar, a lane's part of the address is a constant but in the segment's last step, where keys past
+  // the last one stand for it (addresses by lane: 69.3 -> 67.4 us for one tree of 61 nodes over 32000 keys).
+  constexpr int RW = kWave / CPR, RJ = P::T / CPR;
   u32x4_t kbuf[NLD], vbuf[NLD];
   bool okbuf = true;
-  int bid[NLD];
+  int bid[NLD];  // of the step that is fetched next
+  uint32_t mine[NLD];
+#pragma unroll
+  for (int j = 0; j < NLD; ++j) mine[j] = lane * 16;
+  const int ncb = static_cast<int>(a.ncb), inside = a.bs - 1, w0 = w * RW;
+  const uint32_t per_block = static_cast<uint32_t>(a.hkv * a.bs), head = static_cast<uint32_t>(p.kvh * a.bs);
   auto lookup = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < NLD; ++j) {
-      const int key = t * P::KT + (tid + j * P::T) / CPR;
-      bid[j] = table[(key < last ? key : last) >> a.log2_bs];
+      const int key = t * P::KT + j * RJ + w0;
+      bid[j] = load_uniform_i32(table + ((key < last ? key : last) >> a.log2_bs));
     }
   };
   auto fetch = [&](int t) __attribute__((always_inline)) {
     okbuf = true;
+    const bool whole = t * P::KT + P::KT - 1 <= last;
+    if (!whole) {
+#pragma unroll
+      for (int j = 0; j < NLD; ++j) {
+        const int key = t * P::KT + j * RJ + w0, from = key < last ? key : last;
+        const int mid = key + lane / CPR < last ? key + lane / CPR : last;  // at `from` or behind it, in the same block
+        mine[j] = static_cast<uint32_t>(mid - from) * RB + lane % CPR * 16;
+      }
+      okbuf = false;
+    }
 #pragma unroll
     for (int j = 0; j < NLD; ++j) {
-      const int idx = tid + j * P::T, r = idx / CPR, c = idx % CPR;
-      const int key = t * P::KT + r, kk = key < last ? key : last;  // keys past the last one stand for it
-      const bool bok = bid[j] >= 0 && bid[j] < a.ncb;
-      const uint64_t row = static_cast<uint64_t>(bok ? static_cast<uint32_t>(bid[j]) : 0u) *
-                               static_cast<uint32_t>(a.hkv * a.bs) +
-                           static_cast<uint32_t>(p.kvh * a.bs + (kk & (a.bs - 1)));
-      kbuf[j] = *reinterpret_cast<const u32x4_t*>(a.k + row * RB + c * 16);
-      vbuf[j] = *reinterpret_cast<const u32x4_t*>(a.v + row * RB + c * 16);
-      okbuf = okbuf && bok && key <= last;
+      const int key = t * P::KT + j * RJ + w0, from = key < last ? key : last;
+      const bool bok = bid[j] >= 0 && bid[j] < ncb;
+      const uint64_t row = static_cast<uint64_t>(bok ? static_cast<uint32_t>(bid[j]) : 0u) * per_block +
+                           (head + static_cast<uint32_t>(from & inside));
+      kbuf[j] = *reinterpret_cast<const u32x4_t*>(a.k + row * RB + mine[j]);
+      vbuf[j] = *reinterpret_cast<const u32x4_t*>(a.v + row * RB + mine[j]);
+      okbuf = okbuf && bok;
     }
   };
   auto stash = [&](int stage) __attribute__((always_inline)) {
@@ -647,8 +664,7 @@ __device__ __forceinline__ void shared_pass(const TreeArgs& a, const Piece& p, R
       *reinterpret_cast<u32x4_t*>(st + r * RB + ((c ^ (r & (CPR - 1))) * 16)) = kbuf[j];
       *reinterpret_cast<u32x4_t*>(st + P::TILE + r * RB + ((c ^ vsw<D>(r)) * 16)) = vv;
     }
-    const bool ok = __all(okbuf);
-    if (lane == 0) reinterpret_cast<uint8_t*>(&sh.ok[stage])[w] = ok ? 1 : 0;
+    if (lane == 0) reinterpret_cast<uint8_t*>(&sh.ok[stage])[w] = okbuf ? 1 : 0;
   };
   lookup(p.step0);
   fetch(p.step0);
@@ -1160,23 +1176,23 @@ Config config_of() {
 // The workgroup's shape by the most rows a segment's kv head can have, and the products of the call (sequences x kv
 // heads x rows x keys). Wavefronts with the same 16, 32 or 64 rows and keys of their own need no staging together and
 // cut a segment finely; wavefronts with rows of their own that share keys read each key a quarter as often. The
-// second pays for more rows than 64 once the call is large (graph replay, us, own keys / shared; sequences x nodes of 7
+// second takes blocks of 8 tokens or more and pays for more rows than 64 once the call is large (graph replay, us, own keys / shared; sequences x nodes of 7
 // rows; d64, 2 kv heads: 16 x 24 over 1024 keys 19.1/23.0, 64 x 48 over 256 21.9/29.1, 64 x 24 over 1024 (22M) 28.6/30.8,
 // 64 x 32 over 1024 (29M) 36.7/32.5, 64 x 48 over 1024 43.2/37.9, 64 x 64 over 4096 109/84.7; d128, 4 kv heads: 4 x 24
 // over 4096 28.7/32.6, 1 x 16 over 32768 (15M) 33.4/34.8, 16 x 48 over 1024 (22M) 49.2/41.5, 16 x 64 over 4096 137/83.4).
 // d64 with shared keys: 32 rows a wavefront and three workgroups a CU against 64 and two, 64 x 64 over 512 36.0/39.0,
 // 256 x 64 over 512 66.9/73.2, 64 x 64 over 4096 87.0/85.8.
 template <int DT>
-Config pick(int d, int64_t rows, int64_t products) {
+Config pick(int d, int64_t rows, int64_t products, int bs) {
   if (d == 64) {
     if (rows <= 16) return config_of<DT, 64, 1, 4, 1, 2>();
     if (rows <= 32) return config_of<DT, 64, 1, 4, 2, 2>();
-    if (rows <= 64 || products <= 28 << 20) return config_of<DT, 64, 1, 4, 4, 2>();
+    if (rows <= 64 || products <= 28 << 20 || bs < 8) return config_of<DT, 64, 1, 4, 4, 2>();
     return config_of<DT, 64, 4, 1, 2, 3>();
   }
   if (rows <= 16) return config_of<DT, 128, 1, 4, 1, 1>();
   if (rows <= 32) return config_of<DT, 128, 1, 4, 2, 1>();
-  if (rows <= 64 || products <= 16 << 20) return config_of<DT, 128, 1, 4, 4, 1>();
+  if (rows <= 64 || products <= 16 << 20 || bs < 8) return config_of<DT, 128, 1, 4, 4, 1>();
   return config_of<DT, 128, 4, 1, 2, 2>();
 }
 
@@ -1203,7 +1219,7 @@ Plan plan_of(int num_seqs, int max_q_len, int hq, int hkv, int d, int bs, int ma
   const int64_t rows = static_cast<int64_t>(max_q_len) * group, cap = static_cast<int64_t>(max_blocks) * bs;
   if ((dtype != MIP_F16 && dtype != MIP_BF16) || (d != 64 && d != 128)) return p;
   const int64_t products = static_cast<int64_t>(num_seqs) * hkv * rows * cap;
-  p.cfg = dtype == MIP_F16 ? pick<MIP_F16>(d, rows, products) : pick<MIP_BF16>(d, rows, products);
+  p.cfg = dtype == MIP_F16 ? pick<MIP_F16>(d, rows, products, bs) : pick<MIP_BF16>(d, rows, products, bs);
   const int64_t segs = hkv * ((rows + p.cfg.rows - 1) / p.cfg.rows), steps = (cap + p.cfg.keys - 1) / p.cfg.keys;
   if ((rows + 256) * group >= (int64_t{1} << 31) || segs * steps >= (int64_t{1} << 30) || segs * num_seqs * steps >= (int64_t{1} << 30) ||
       segs * num_seqs >= (int64_t{1} << 24))

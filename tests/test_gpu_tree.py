@@ -185,6 +185,81 @@ def test_large_values(gpu, dtype, nodes):
     step.check(run(gpu, step))
 
 
+def widened(step, args):
+    """``args`` with tables so wide (their further entries are no blocks) that the call is taken for a large one: its rows
+    of more than 64 then run on wavefronts that share their keys."""
+    rows = step.most * (step.hq // step.hkv)
+    assert rows > 64 and step.bs >= 8
+    width = -(-(32 << 20) // (len(step.nodes) * step.hkv * rows * step.bs)) + step.width()
+    tab = torch.full((len(step.nodes), width), -1, dtype=torch.int32, device=args["block_tables"].device)
+    tab[:, :args["block_tables"].shape[1]] = args["block_tables"]
+    return {**args, "block_tables": tab}
+
+
+LARGE = [(64, 14, 2, 16), (128, 28, 4, 32), (64, 8, 1, 8), (128, 16, 1, 8), (64, 40, 2, 64)]
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("d,hq,hkv,bs", LARGE)
+@pytest.mark.parametrize("starts,nodes,kind", [
+    ([300], [20], "tree"), ([0, 3, 64], [20, 1, 33], "tree"), ([130, 0, 31, 512, 257], [30, 20, 0, 17, 2], "tree"),
+    ([0, 17], [70, 130], "free"), ([2222], [40], "chain")])
+def test_large_calls_match_f64(gpu, dtype, d, hq, hkv, bs, starts, nodes, kind):
+    announce(f"paged_tree large call {dtype} d={d} hq={hq} hkv={hkv} bs={bs} starts={starts} nodes={nodes} {kind}")
+    step = Step(dtype, d, hq, hkv, bs, starts, nodes, seed=len(starts) + 20, kind=kind)
+    step.check(run(gpu, step, **widened(step, step.to(gpu))))
+
+
+@pytest.mark.parametrize("d,hq,hkv,bs", [(64, 14, 2, 8), (128, 28, 4, 16)])
+def test_large_calls_at_every_end(gpu, d, hq, hkv, bs):
+    """Contexts that end at every place of a step of 32 keys and of a block, in one batch."""
+    announce(f"paged_tree large call, every end d={d}")
+    step = Step("bfloat16", d, hq, hkv, bs, list(range(40, 74)), [12] * 34, seed=31)
+    step.check(run(gpu, step, **widened(step, step.to(gpu))))
+
+
+@pytest.mark.parametrize("d,bs", [(64, 16), (128, 8)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_large_calls_what_a_row_does_not_see_has_no_influence(gpu, d, bs, bad):
+    announce(f"paged_tree large call masked {bad} d={d}")
+    step = Step("bfloat16", d, 28, 4, bs, [45, 300], [20, 9], seed=11)
+    step.tables[1][3] = -7  # a block outside the pool
+    leaf = 19
+    for x in (step.k, step.v):
+        x[step.tables[0][(45 + leaf) // bs], :, (45 + leaf) % bs] = bad
+        x[step.tables[1][-1], :, 309 - (len(step.tables[1]) - 1) * bs:] = bad
+    got = run(gpu, step, **widened(step, step.to(gpu))).double().cpu().numpy()
+    with np.errstate(invalid="ignore"):
+        out, _, _ = step.want()
+    keep = [i for i in range(29) if i != leaf]
+    assert np.isfinite(out[keep]).all() and np.abs(got[keep] - out[keep]).max() <= 2e-2  # 8 half steps of values of order one
+
+
+@pytest.mark.parametrize("d,hq,hkv", [(64, 14, 2), (128, 28, 4)])
+@pytest.mark.parametrize("scale", [2.0**-30, 1.0, 2.0**100])
+def test_large_calls_with_small_and_large_values(gpu, d, hq, hkv, scale):
+    """bf16 values that fp16 does not hold: everywhere, and in one dim of ordinary ones."""
+    announce(f"paged_tree large call values of {scale} d={d}")
+    step = Step("bfloat16", d, hq, hkv, 16, [300, 50], [12, 20], seed=33)
+    step.v *= scale
+    step.v[..., 9] *= 2.0**-30
+    got = run(gpu, step, **widened(step, step.to(gpu))).double().cpu().numpy()
+    out, spread, reach = step.want()
+    delta = (d + 2) * 2.0**-24 * reach + 2.0**-21 + 400 * 2.0**-23 + 2.0**-11
+    bound = 2.0**-8 * 1.01 * np.abs(out) + 2.05 * delta[..., None] * spread + 400 * 2.0**-31 * spread
+    assert (np.abs(got - out) <= bound)[..., 9].all()
+    if scale != 1.0:
+        assert (np.abs(got - out) <= bound).all()
+    step.check(torch.from_numpy(got))
+
+
+def test_a_tree_of_a_thousand_nodes(gpu):
+    announce("paged_tree 1024 nodes")
+    for dtype, d, hq in (("bfloat16", 64, 4), ("float32", 64, 2)):
+        step = Step(dtype, d, hq, 2, 16, [21], [1024], seed=34)
+        step.check(run(gpu, step))
+
+
 @pytest.mark.parametrize("dtype,d,hq,hkv,nodes", [
     ("bfloat16", 64, 14, 2, [3, 12]), ("bfloat16", 64, 14, 2, [40, 5]), ("bfloat16", 128, 28, 4, [12]), ("bfloat16", 64, 14, 2, [2]),
     ("float32", 64, 14, 2, [12]), ("bfloat16", 32, 14, 2, [12])])
