@@ -736,11 +736,11 @@ def copy_blocks(k_pool: torch.Tensor, v_pool: torch.Tensor, pairs) -> None:
 
 def _one_device(*tensors: torch.Tensor) -> torch.device:
     """The device that all of these are on; a call whose pointers belong to several is refused."""
-    device = tensors[0].device
+    device, index = tensors[0].device, tensors[0].get_device()
     for t in tensors:
-        if t.device != device:
+        if t.get_device() != index or (index < 0 and t.device != device):
             raise ValueError(f"tensors on different devices: {device} and {t.device}")
-    if device.type != "cuda":
+    if not tensors[0].is_cuda:
         _require_device(tensors[0])
     return device
 
@@ -756,23 +756,27 @@ def _call_on(device: torch.device, fn, args: tuple, what: str) -> None:
         _native.check(st, what)
 
 
+_I32 = torch.int32
+
+
 def _tree_rows(cu_q: torch.Tensor, block_tables: torch.Tensor, ctx_start: torch.Tensor, max_q_len: int,
                max_blocks: int | None) -> tuple[int, int]:
     """Check the tensors that describe a step of trees; returns (sequences, blocks of a table)."""
-    if not cu_q.dtype == ctx_start.dtype == block_tables.dtype == torch.int32:
+    if not cu_q.dtype == ctx_start.dtype == block_tables.dtype == _I32:
         raise TypeError("cu_q, ctx_start and block_tables must be int32")
-    if ctx_start.dim() != 1 or cu_q.shape != (ctx_start.shape[0] + 1,):
+    seqs, tab = ctx_start.shape, block_tables.shape
+    if len(seqs) != 1 or cu_q.shape != (seqs[0] + 1,):
         raise ValueError("cu_q must be int32 [S + 1] and ctx_start int32 [S]")
-    s = ctx_start.shape[0]
-    if block_tables.dim() != 2 or block_tables.shape[0] < s or block_tables.shape[1] < 1:
+    s = seqs[0]
+    if len(tab) != 2 or tab[0] < s or tab[1] < 1:
         raise ValueError("block_tables must be int32 [S, max_blocks]")
     if not (cu_q.is_contiguous() and ctx_start.is_contiguous()) or block_tables.stride(1) != 1:
         raise ValueError("cu_q, ctx_start and the block_tables rows must be contiguous")
     if max_q_len < 0:
         raise ValueError(f"max_q_len={max_q_len} is negative")
-    mb = block_tables.shape[1] if max_blocks is None else int(max_blocks)
-    if mb < 1 or mb > block_tables.shape[1]:
-        raise ValueError(f"max_blocks={mb} is outside [1, {block_tables.shape[1]}]")
+    mb = tab[1] if max_blocks is None else int(max_blocks)
+    if mb < 1 or mb > tab[1]:
+        raise ValueError(f"max_blocks={mb} is outside [1, {tab[1]}]")
     return s, mb
 
 
@@ -820,11 +824,11 @@ def tree_index(parents: torch.Tensor, cu_q: torch.Tensor, ctx_start: torch.Tenso
     padded batch's, and a tree's from ``max_q_len`` on) have position 0, slot -1 and no bits.
     """
     s, mb = _tree_rows(cu_q, block_tables, ctx_start, max_q_len, max_blocks)
-    if parents.dtype != torch.int32 or parents.dim() != 1 or not parents.is_contiguous():
+    if parents.dtype != _I32 or parents.dim() != 1 or not parents.is_contiguous():
         raise ValueError("parents must be contiguous int32 [N]")
     device = _one_device(parents, cu_q, ctx_start, block_tables)
     n, words = parents.shape[0], (max_q_len + 63) // 64
-    positions = torch.empty(n, dtype=torch.int64, device=device)
+    positions = parents.new_empty(n, dtype=torch.int64)
     slots, mask = torch.empty_like(positions), positions.new_empty(n, words)
     if n:
         _call_on(device, _native.load().mip_tree_index,
@@ -840,38 +844,43 @@ def _tree_args(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
                workspace: torch.Tensor | None) -> tuple[tuple | None, torch.Tensor, torch.Tensor | None]:
     """Validate a :func:`paged_tree` call: the arguments of ``mip_paged_tree`` up to the stream (None for a call that
     has nothing to do), the output and the scratch memory."""
-    if q.dim() != 3 or q.stride(2) != 1:
+    rows, pool, strides = q.shape, k_cache.shape, q.stride()
+    if len(rows) != 3 or strides[2] != 1:
         raise ValueError("q must be [N, Hq, D] with a contiguous last dimension")
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+    if len(pool) != 4 or pool != v_cache.shape or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError("k_cache/v_cache must be contiguous [num_blocks, Hkv, block_size, D] tensors of one shape")
-    nb, hkv, bs, d = k_cache.shape
-    n, hq, dq = q.shape
+    nb, hkv, bs, d = pool
+    n, hq, dq = rows
     if dq != d or hkv == 0 or hq == 0 or hq % hkv:
-        raise ValueError(f"q {tuple(q.shape)} does not match the pool (Hkv={hkv}, D={d})")
-    if q.dtype != k_cache.dtype or v_cache.dtype != k_cache.dtype:
+        raise ValueError(f"q {tuple(rows)} does not match the pool (Hkv={hkv}, D={d})")
+    dtype = q.dtype
+    if not dtype == k_cache.dtype == v_cache.dtype:
         raise TypeError("q and the cache must share one dtype")
     s, mb = _tree_rows(cu_q, block_tables, ctx_start, max_q_len, max_blocks)
-    words = (max_q_len + 63) // 64
-    if mask.dtype != torch.int64 or mask.dim() != 2 or mask.shape[0] != n or mask.shape[1] < words or (
-            mask.shape[1] > 1 and mask.stride(1) != 1):
-        raise ValueError(f"mask must be int64 [{n}, >= {words}] with contiguous rows, got {tuple(mask.shape)} {mask.dtype}")
+    words, bits, bit_strides = (max_q_len + 63) // 64, mask.shape, mask.stride()
+    if mask.dtype != torch.int64 or len(bits) != 2 or bits[0] != n or bits[1] < words or (
+            bits[1] > 1 and bit_strides[1] != 1):
+        raise ValueError(f"mask must be int64 [{n}, >= {words}] with contiguous rows, got {tuple(bits)} {mask.dtype}")
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     if not 0.0 < scale < math.inf:
         raise ValueError(f"scale={scale} must be positive")
     if out is None:
-        out = q.new_empty(n, hq, d)
-    elif out.shape != (n, hq, d) or out.dtype != q.dtype or out.stride(2) != 1:
-        raise ValueError("out must be [N, Hq, D] in q's dtype with a contiguous last dimension")
-    device = _one_device(q, k_cache, v_cache, block_tables, cu_q, ctx_start, mask, out)
+        device = _one_device(q, k_cache, v_cache, block_tables, cu_q, ctx_start, mask)
+        out, to = torch.empty_like(q, memory_format=torch.contiguous_format), (hq * d, d)
+    else:
+        to = out.stride()
+        if out.shape != rows or out.dtype != dtype or to[2] != 1:
+            raise ValueError("out must be [N, Hq, D] in q's dtype with a contiguous last dimension")
+        device = _one_device(q, k_cache, v_cache, block_tables, cu_q, ctx_start, mask, out)
     if not (n and s and max_q_len):
         return None, out, None
-    code = dtype_code(q.dtype)
+    code = dtype_code(dtype)
     workspace = _scratch(workspace, device, _tree_bytes(device, s, max_q_len, hq, hkv, d, bs, mb, code))
     ws_ptr, ws_bytes = _extent(workspace)
-    return (out.data_ptr(), out.stride(0), out.stride(1), q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
+    return (out.data_ptr(), to[0], to[1], q.data_ptr(), strides[0], strides[1], k_cache.data_ptr(),
             v_cache.data_ptr(), nb, block_tables.data_ptr(), block_tables.stride(0), cu_q.data_ptr(),
-            ctx_start.data_ptr(), mask.data_ptr(), max(mask.stride(0), mask.shape[1]) if n == 1 else mask.stride(0),
-            mask.shape[1], s, max_q_len, hq, hkv, d, bs, mb, scale, ws_ptr, ws_bytes, code), out, workspace
+            ctx_start.data_ptr(), mask.data_ptr(), max(bit_strides[0], bits[1]) if n == 1 else bit_strides[0],
+            bits[1], s, max_q_len, hq, hkv, d, bs, mb, scale, ws_ptr, ws_bytes, code), out, workspace
 
 
 def paged_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -953,19 +962,20 @@ def tree_verify(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
     ``counts`` (int32 ``[S]``) are the paths' lengths and ``next_token`` (int64 ``[S]``) the target of each one's last node
     (an empty tree: 0 and -1). Scratch memory as for :func:`paged_tree`.
     """
-    if logits.dim() != 2 or logits.shape[1] < 1 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+    rows, strides, seqs = logits.shape, logits.stride(), cu_q.shape
+    if len(rows) != 2 or rows[1] < 1 or (rows[1] > 1 and strides[1] != 1):
         raise ValueError("logits must be [N, vocab] with contiguous rows")
-    n, vocab = logits.shape
+    n, vocab = rows
     code = dtype_code(logits.dtype)
-    if tokens.dtype != torch.int64 or tokens.shape != (n,) or not tokens.is_contiguous():
+    if tokens.dtype != torch.int64 or tokens.shape != rows[:1] or not tokens.is_contiguous():
         raise ValueError(f"tokens must be contiguous int64 [{n}]")
-    if parents.dtype != torch.int32 or parents.shape != (n,) or not parents.is_contiguous():
+    if parents.dtype != _I32 or parents.shape != rows[:1] or not parents.is_contiguous():
         raise ValueError(f"parents must be contiguous int32 [{n}]")
-    if cu_q.dtype != torch.int32 or cu_q.dim() != 1 or cu_q.shape[0] < 1 or not cu_q.is_contiguous():
+    if cu_q.dtype != _I32 or len(seqs) != 1 or seqs[0] < 1 or not cu_q.is_contiguous():
         raise ValueError("cu_q must be contiguous int32 [S + 1]")
     if max_q_len < 0:
         raise ValueError(f"max_q_len={max_q_len} is negative")
-    s, row_stride = cu_q.shape[0] - 1, max(logits.stride(0), vocab) if n <= 1 else logits.stride(0)
+    s, row_stride = seqs[0] - 1, max(strides[0], vocab) if n <= 1 else strides[0]
     if row_stride < vocab:
         raise ValueError("the rows of logits overlap")
     device = _one_device(logits, tokens, parents, cu_q)
@@ -993,29 +1003,31 @@ def tree_commit(k_pool: torch.Tensor, v_pool: torch.Tensor, block_tables: torch.
     No two sequences may own the blocks that rows move in (a block that a fork shares is copied before the nodes are
     appended: ``PagedKVCache.prepare_writes``).
     """
-    if k_pool.dim() != 5 or k_pool.shape != v_pool.shape or not (k_pool.is_contiguous() and v_pool.is_contiguous()):
+    pool, dtype = k_pool.shape, k_pool.dtype
+    if len(pool) != 5 or pool != v_pool.shape or not (k_pool.is_contiguous() and v_pool.is_contiguous()):
         raise ValueError("k_pool/v_pool must be contiguous [L, num_blocks, Hkv, block_size, D] tensors of one shape")
-    if k_pool.dtype != v_pool.dtype:
+    if dtype != v_pool.dtype:
         raise TypeError("the pools must share one dtype")
-    if not path.dtype == counts.dtype == ctx_start.dtype == block_tables.dtype == torch.int32:
+    if not path.dtype == counts.dtype == ctx_start.dtype == block_tables.dtype == _I32:
         raise TypeError("path, counts, ctx_start and block_tables must be int32")
-    s = counts.numel()
-    if counts.dim() != 1 or ctx_start.shape != (s,) or path.dim() != 2 or path.shape[0] != s:
+    seqs, steps, tab, step, row = counts.shape, path.shape, block_tables.shape, path.stride(), block_tables.stride()
+    if len(seqs) != 1 or ctx_start.shape != seqs or len(steps) != 2 or steps[0] != seqs[0]:
         raise ValueError("path must be int32 [S, P], counts and ctx_start int32 [S]")
-    if block_tables.dim() != 2 or block_tables.shape[0] < s or block_tables.shape[1] < 1 or block_tables.stride(1) != 1:
+    s, most = steps
+    if len(tab) != 2 or tab[0] < s or tab[1] < 1 or row[1] != 1:
         raise ValueError("block_tables must be int32 [S, max_blocks] with contiguous rows")
-    if not (counts.is_contiguous() and ctx_start.is_contiguous()) or (path.shape[1] > 1 and path.stride(1) != 1) or (
-            s > 1 and path.stride(0) < path.shape[1]):
+    if not (counts.is_contiguous() and ctx_start.is_contiguous()) or (most > 1 and step[1] != 1) or (
+            s > 1 and step[0] < most):
         raise ValueError("counts, ctx_start and the rows of path must be contiguous")
-    mb = block_tables.shape[1] if max_blocks is None else int(max_blocks)
-    if mb < 1 or mb > block_tables.shape[1]:
-        raise ValueError(f"max_blocks={mb} is outside [1, {block_tables.shape[1]}]")
-    layers, nb, hkv, bs, d = k_pool.shape
-    code = dtype_code(k_pool.dtype)
+    mb = tab[1] if max_blocks is None else int(max_blocks)
+    if mb < 1 or mb > tab[1]:
+        raise ValueError(f"max_blocks={mb} is outside [1, {tab[1]}]")
+    layers, nb, hkv, bs, d = pool
+    code = dtype_code(dtype)
     device = _one_device(k_pool, v_pool, block_tables, ctx_start, path, counts)
-    if s == 0 or path.shape[1] == 0:
+    if s == 0 or most == 0:
         return
     _call_on(device, _native.load().mip_tree_commit,
              (k_pool.data_ptr(), v_pool.data_ptr(), layers, nb, hkv, d, bs, block_tables.data_ptr(),
-              block_tables.stride(0), mb, ctx_start.data_ptr(), path.data_ptr(), max(path.stride(0), path.shape[1]),
-              path.shape[1], counts.data_ptr(), s, code), "mip_tree_commit")
+              row[0], mb, ctx_start.data_ptr(), path.data_ptr(), max(step[0], most), most, counts.data_ptr(), s, code),
+             "mip_tree_commit")
