@@ -45,8 +45,8 @@
 // must not reach a row as 0 * inf.
 //
 // Measured (graph replay, us a call, both kernels): 128 sequences of 4-8 nodes, 28q/4kv d128, 512-8192
-// keys: 171, 725 MB at 4.2 TB/s; 64 x 33-64 nodes, 14q/2kv d64, 128-4096 keys: 51, 231 TFLOP/s; 61 nodes over
-// 32000 keys, 28q/4kv d128: 65, 430 TFLOP/s; 32 x 8-24 nodes, 128-1024 keys: 20; 5 nodes over 37 keys: 4.0.
+// keys: 171, 725 MB at 4.2 TB/s; 64 x 33-64 nodes, 14q/2kv d64, 128-4096 keys: 50, 234 TFLOP/s; 61 nodes over
+// 32000 keys, 28q/4kv d128: 66, 422 TFLOP/s; 32 x 8-24 nodes, 128-1024 keys: 19; 5 nodes over 37 keys: 4.0.
 #include "paged_decode_common.h"
 
 namespace mip {
@@ -1229,12 +1229,15 @@ Plan plan_of(int num_seqs, int max_q_len, int hq, int hkv, int d, int bs, int ma
   p.min_share = (kMinShareKeys + p.cfg.keys - 1) / p.cfg.keys;
   const int64_t most = (segs * num_seqs * steps + p.min_share - 1) / p.min_share, slots = compute_units() * p.cfg.occ;
   p.grid = static_cast<int>((most < slots ? most : slots) + 7) / 8 * 8;
-  // Short segments are left whole where there are enough of them for the chip (graph replay, us, cut / whole;
-  // sequences x nodes over 256-512 keys, 14q/2kv d64: 64 x 2 11.0/10.6, 64 x 8 17.3/15.4, 256 x 4 23.5/18.6, 256 x 64
-  // 82.1/70.6; 28q/4kv d128 over 512-1024: 16 x 8 24.6/22.2, 64 x 8 46.4/43.7) and cut where there are few (64 nodes
-  // over 250 keys 13.6/18.8; 4 x 64 over 512 16.2/23.9; d128 4 x 8 15.7/17.5, 64 x 16 41.3/47.9).
+  // Where there are enough segments for the chip, cuts keep away from their ends, and segments of up to 640 keys stay
+  // whole, at which no second kernel is launched (graph replay, us, cut anywhere / 256 keys away / 384; sequences x
+  // nodes over half of to all of the keys, 14q/2kv d64, 512 keys: 32 x 24 20.6/19.5/16.2, 64 x 12 21.3/19.6/16.8, 128 x 12
+  // 28.2/23.4/18.3; 1024: 32 x 12 20.3/18.9/22.5, 32 x 24 24.9/22.1/25.3, 64 x 5 18.9/18.0/21.0, 64 x 24 30.9/29.9/28.4;
+  // 2048: 32 x 12 25.3/22.7/23.6, 64 x 12 31.2/29.9/30.4; 28q/4kv d128, 512 keys, cut / 256 away / whole: 32 x 5
+  // 22.9/20.1/16.6, 32 x 12 29.6/25.1/20.1; 1024: 8 x 12 22.5/20.3). Where there are few, they are cut anywhere (64
+  // nodes over 250 keys 13.6, whole 18.8; 4 x 64 over 512 16.2/23.9).
   const int64_t all = segs * num_seqs;
-  if (p.cfg.keys >= 128 ? 4 * all >= p.grid : all >= 2 * p.grid) p.slack = (d == 64 ? 384 : 256) / p.cfg.keys;
+  if (p.cfg.keys >= 128 ? 4 * all >= p.grid : all >= 2 * p.grid) p.slack = (cap <= 640 ? 384 : 256) / p.cfg.keys;
   if (steps >= 2 * p.slack) {  // else no cut stays inside a segment
     p.start_off = (static_cast<int64_t>(p.grid) * 2 * p.cfg.rec_floats * 4 + 255) / 256 * 256;
     p.bytes = p.start_off + (num_seqs + 1) * 4;
