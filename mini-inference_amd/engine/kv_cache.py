@@ -685,6 +685,8 @@ class PagedTreeContext:
                 raise ValueError("every tree needs a root, and a token and a parent for each node")
             if tree[0] != -1 or any(not 0 <= p < i for i, p in enumerate(tree) if i):
                 raise ValueError("node 0 is the root (parent -1) and every other node's parent comes before it")
+            if min(toks) < 0:  # a padded draft: no embedding has such a row
+                raise ValueError(f"token {min(toks)} is negative; leave a draft's missing nodes out")
         self.lengths = [len(t) for t in tokens]
         self.max_q_len = max(self.lengths)
         if self.max_q_len > paged_ops.MAX_TREE_NODES:

@@ -188,6 +188,7 @@ def small_cache(max_len=64):
     ([0], [[1, 2]], [[0, -1]], "node 0 is the root"),
     ([0], [[1, 2]], [[-1, -1]], "node 0 is the root"),
     ([0], [[1, 2, 3]], [[-1, 2, 0]], "comes before"),
+    ([0], [[1, 2, -1]], [[-1, 0, 1]], "negative"),
     ([0], [[0] * 1025], [[-1] + [0] * 1024], "at most 1024"),
 ])
 def test_tree_context_refuses(slots, tokens, parents, match):
