@@ -910,7 +910,10 @@ def paged_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
 
 
 class TreeStepCalls(PrefillStepCalls):
-    """The layer calls of one step of drafted trees; the nodes are appended as a packed prefill's tokens are."""
+    """The layer calls of one step of drafted trees; the nodes are appended as a packed prefill's tokens are.
+
+    The calls of a step share one piece of scratch memory, which the first of them allocates: they belong on one stream,
+    or into one graph, in order, as a model issues them."""
 
     def __init__(self, block_tables: torch.Tensor, cu_q: torch.Tensor, ctx_start: torch.Tensor, mask: torch.Tensor,
                  slot_mapping: torch.Tensor, max_q_len: int, scale: float) -> None:

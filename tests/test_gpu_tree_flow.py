@@ -219,3 +219,43 @@ def test_layer_calls_that_change_layout_are_checked_again(gpu):
                                     ctx.ctx_start, ctx.mask, 3)
         torch.cuda.synchronize()
         assert out.shape == (1, 6, 3, 64) and torch.equal(out[0].transpose(0, 1), want)
+
+
+@torch.inference_mode()
+def test_captured_layer_calls_replay_on_new_inputs(gpu):
+    """A step's layer calls in a graph (long context: scratch memory in use): every replay equals the eager calls on
+    what the buffers hold then, eager calls of the same step between the replays."""
+    from engine.kv_cache import PagedKVCache
+
+    announce("captured tree layer calls")
+    cache = PagedKVCache(2, 2, 64, num_blocks=300, block_size=16, max_seqs=2, max_len=4600, dtype=torch.bfloat16, device=gpu)
+    slot = cache.allocate(4500)
+    cache.lengths[slot] = 4500
+    cache.k.normal_()
+    cache.v.normal_()
+    ctx = cache.tree_context([slot], [[1] * 9], [[-1, 0, 0, 1, 1, 2, 3, 4, 4]])
+    q = torch.randn(2, 1, 9, 14, 64, device=gpu).bfloat16().transpose(2, 3)
+    k, v = (torch.randn(2, 1, 9, 2, 64, device=gpu).bfloat16().transpose(2, 3) for _ in range(2))
+
+    def work():
+        return [ctx.attend(layer, q[layer], k[layer], v[layer]) for layer in range(2)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = work()
+    for seed in range(4):
+        gen = torch.Generator(device=gpu).manual_seed(seed)
+        for x in (q, k, v):
+            x.normal_(generator=gen)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [x.clone() for x in outs]
+        want = work()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+        assert float(got[0].float().abs().max()) > 0
