@@ -23,7 +23,7 @@ from __future__ import annotations
 import math
 import random
 import sys
-from functools import lru_cache, reduce
+from functools import reduce
 from pathlib import Path
 
 import torch
@@ -303,9 +303,8 @@ def _plain_commit(st):
 
 
 # ---------------------------------------------------------------------------------- one pass
-@lru_cache(None)
 def _ops():
-    """The framework's tensor-level entry points, imported once as a program does."""
+    """The framework's tensor-level entry points."""
     package = str(Path(__file__).resolve().parent.parent / "mini-inference_amd")
     if package not in sys.path:
         sys.path.insert(0, package)
