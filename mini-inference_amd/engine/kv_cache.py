@@ -216,9 +216,31 @@ class PagedKVCache:
         reference count is above one is replaced in that sequence's table by a fresh block,
         and one :meth:`copy_blocks` call copies all of them (all layers, K and V; one launch
         per 128 pairs).
-        Returns the ``(src, dst)`` pairs copied. Raises if the pool cannot supply them.
+        Returns the ``(src, dst)`` pairs copied. Raises, with no table changed, if the pool cannot supply them all.
         """
+        shared = self._shared_writes(slots, starts, counts)
+        if len(shared) > len(self._free_blocks):
+            raise RuntimeError("not enough free KV cache blocks for copy-on-write")
         pairs: list[tuple[int, int]] = []
+        for slot, i, old in shared:
+            new = self._new_block()
+            self.block_tables[slot][i] = new
+            self._release(old)
+            pairs.append((old, new))
+            if self._journal is not None:
+                self._journal.append((slot, i, new))
+        if pairs:
+            self.copy_blocks(pairs)
+            self.cow_copies += len(pairs)
+        return pairs
+
+    def _shared_writes(self, slots: Sequence[int], starts: Sequence[int],
+                       counts: Sequence[int]) -> list[tuple[int, int, int]]:
+        """``(slot, index, block)`` of the table entries that these writes need private copies for.
+
+        Of the sequences that share a block the last one to be left with it keeps it."""
+        found: dict[tuple[int, int], int] = {}
+        left: dict[int, int] = {}  # references a block has once the copies found so far are made
         bs, refs, tables = self.block_size, self._ref_counts, self.block_tables
         for slot, start, n in zip(slots, starts, counts):
             if n <= 0:
@@ -228,22 +250,12 @@ class PagedKVCache:
             last = (start + n - 1) // bs
             if first == last < len(table) and refs[table[first]] <= 1:
                 continue  # one block, already private: the usual decode write
-            last = min(last, len(table) - 1)
-            for i in range(first, last + 1):
+            for i in range(first, min(last, len(table) - 1) + 1):
                 old = table[i]
-                if refs[old] > 1:
-                    if not self._free_blocks:
-                        raise RuntimeError("not enough free KV cache blocks for copy-on-write")
-                    new = self._new_block()
-                    table[i] = new
-                    self._release(old)
-                    pairs.append((old, new))
-                    if self._journal is not None:
-                        self._journal.append((slot, i, new))
-        if pairs:
-            self.copy_blocks(pairs)
-            self.cow_copies += len(pairs)
-        return pairs
+                if left.get(old, refs[old]) > 1 and (slot, i) not in found:
+                    left[old] = left.get(old, refs[old]) - 1
+                    found[slot, i] = old
+        return [(slot, i, old) for (slot, i), old in found.items()]
 
     def copy_blocks(self, pairs: Sequence[tuple[int, int]] | torch.Tensor) -> None:
         """``k[:, dst] = k[:, src]`` and ``v[:, dst] = v[:, src]`` for every (src, dst), all layers, on device.
