@@ -676,8 +676,9 @@ class PagedTreeContext:
 
     Node i is stored behind the cached tokens in its own place (``slot_mapping``), whatever its depth, and sees the cached
     tokens and its own path (``mask``); accepting a path moves its rows to consecutive places. The blocks for all
-    nodes are allocated, and shared ones copied, when the context is made; those that the accepted path does not fill
-    stay with the sequence for its next tokens.
+    nodes are allocated, and shared ones copied, when the context is made (a step that the pool or ``max_len`` has no
+    room for is refused and takes none); those that the accepted path does not fill stay with the sequence for its
+    next tokens.
     """
 
     fuse_rope = True
@@ -707,16 +708,22 @@ class PagedTreeContext:
         self.tokens = [list(t) for t in tokens]
         self.starts = [cache.lengths[s] for s in self.slots]
         ends = [a + n for a, n in zip(self.starts, self.lengths)]
+        s_n, n, nb = len(self.slots), sum(self.lengths), max(1, cache.blocks_for(max(ends)))
+        ids = np.fromiter(chain.from_iterable(self.tokens), dtype=np.int64, count=n)
+        # All of the step's blocks or none: a refused step leaves the pool as it was.
+        missing = sum(max(0, cache.blocks_for(end) - len(cache.block_tables[s])) for s, end in zip(self.slots, ends))
+        if max(ends) > cache.max_len or missing > cache.num_free_blocks:
+            raise ValueError(f"no room in the KV cache for {n} nodes behind {sum(self.starts)} tokens")
+        if missing + len(cache._shared_writes(self.slots, self.starts, self.lengths)) > cache.num_free_blocks:
+            raise RuntimeError("not enough free KV cache blocks for copy-on-write")
         for s, end in zip(self.slots, ends):
-            if not cache.ensure_capacity(s, end):
-                raise ValueError(f"no room in the KV cache for {end} tokens")
+            cache.ensure_capacity(s, end)
         cache.prepare_writes(self.slots, self.starts, self.lengths)
         dev = cache.k.device
-        s_n, n, nb = len(self.slots), sum(self.lengths), max(1, cache.blocks_for(max(ends)))
         # One upload: tokens (int64) | row offsets | cached lengths | parents | tables (int32).
         n32 = 2 * s_n + 1 + n + s_n * nb
         host = torch.empty(n + (n32 + 1) // 2, dtype=torch.int64, pin_memory=dev.type == "cuda")
-        host.numpy()[:n] = np.fromiter(chain.from_iterable(self.tokens), dtype=np.int64, count=n)
+        host.numpy()[:n] = ids
         i32 = host.numpy()[n:].view(np.int32)
         i32[0] = 0
         np.cumsum(self.lengths, out=i32[1:s_n + 1])
@@ -726,8 +733,8 @@ class PagedTreeContext:
         tables = i32[at + n:n32].reshape(s_n, nb)
         tables.fill(0)
         for row, s in zip(tables, self.slots):
-            ids = cache.block_tables[s][:nb]
-            row[:len(ids)] = ids
+            blocks = cache.block_tables[s][:nb]
+            row[:len(blocks)] = blocks
         i32[n32:] = 0
         on_dev = host.to(dev, non_blocking=True)
         self.input_ids, d32 = on_dev[:n], on_dev[n:].view(torch.int32)

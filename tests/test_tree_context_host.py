@@ -1,0 +1,96 @@
+"""What a drafted-tree step does to the cache's bookkeeping, on the CPU (the kernels' calls replaced)."""
+
+from __future__ import annotations
+
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from engine import paged_ops
+from engine.kv_cache import PagedKVCache
+
+
+@pytest.fixture
+def host(monkeypatch):
+    """Tree contexts on host tensors: the index is blank, and the pool's moves and copies are noted instead of made."""
+    noted = SimpleNamespace(moves=[], copies=[])
+
+    def index(parents, cu_q, ctx_start, tables, max_q_len, block_size):
+        n = parents.shape[0]
+        return torch.zeros(n, dtype=torch.int64), torch.zeros(n, dtype=torch.int64), torch.zeros(n, 1, dtype=torch.int64)
+
+    monkeypatch.setattr(paged_ops, "_require_device", lambda *tensors: None)
+    monkeypatch.setattr(paged_ops, "tree_index", index)
+    monkeypatch.setattr(paged_ops, "tree_commit", lambda *args: noted.moves.append(args))
+    monkeypatch.setattr(paged_ops, "copy_blocks", lambda k, v, pairs: noted.copies.extend(pairs))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: SimpleNamespace(synchronize=lambda: None))
+    return noted
+
+
+def make_cache(num_blocks=4, max_len=64):
+    return PagedKVCache(1, 2, 16, num_blocks=num_blocks, block_size=4, max_seqs=6, max_len=max_len, dtype=torch.float32,
+                        device="cpu")
+
+
+def sequence(cache, tokens):
+    slot = cache.allocate(tokens)
+    cache.lengths[slot] = tokens
+    return slot
+
+
+def state(cache):
+    return ({s: list(t) for s, t in cache.block_tables.items()}, dict(cache.lengths), list(cache._free_blocks),
+            list(cache._ref_counts), cache.cow_copies, None if cache._journal is None else list(cache._journal))
+
+
+def chain(n):
+    return list(range(1, n + 1)), list(range(-1, n - 1))
+
+
+@pytest.mark.parametrize("mirror", [False, True])
+def test_a_refused_step_takes_no_blocks(host, mirror):
+    """Two sequences whose trees fit one at a time: the refusal leaves the blocks, and a decode step for both fits."""
+    cache = make_cache()
+    a, b = sequence(cache, 4), sequence(cache, 4)
+    if mirror:
+        cache.enable_device_tables()
+    before = state(cache)
+    tokens, parents = chain(8)
+    with pytest.raises(ValueError, match="no room"):
+        cache.tree_context([a, b], [tokens, tokens], [parents, parents])
+    assert state(cache) == before
+    assert cache.ensure_capacity(a, 5) and cache.ensure_capacity(b, 5)
+
+
+def test_a_step_refused_by_the_length_limit_takes_no_blocks(host):
+    cache = make_cache(num_blocks=8, max_len=12)
+    a, b = sequence(cache, 4), sequence(cache, 8)
+    before = state(cache)
+    with pytest.raises(ValueError, match="no room"):
+        cache.tree_context([a, b], [chain(8)[0], chain(5)[0]], [chain(8)[1], chain(5)[1]])
+    assert state(cache) == before
+
+
+def test_a_step_refused_for_its_copies_takes_no_blocks(host):
+    """The nodes' own blocks are there, those of the shared partial block's copy are not."""
+    cache = make_cache(num_blocks=4)
+    a = sequence(cache, 6)
+    child = cache.fork(a)
+    before = state(cache)
+    tokens, parents = chain(10)  # two blocks beside the shared one, which takes a third
+    with pytest.raises(RuntimeError, match="copy-on-write"):
+        cache.tree_context([child], [tokens], [parents])
+    assert state(cache) == before and not host.copies
+    ctx = cache.tree_context([child], [tokens[:6]], [parents[:6]])
+    assert len(host.copies) == cache.cow_copies == 1 and cache.num_free_blocks == 0
+    assert ctx.starts == [6] and len(cache.block_tables[child]) == 3
+
+
+def test_a_token_that_no_index_holds_takes_no_blocks(host):
+    cache = make_cache()
+    a = sequence(cache, 4)
+    before = state(cache)
+    with pytest.raises(OverflowError):
+        cache.tree_context([a], [[1, 1 << 70]], [[-1, 0]])
+    assert state(cache) == before
