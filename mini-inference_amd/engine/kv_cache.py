@@ -705,7 +705,7 @@ class PagedTreeContext:
         if self.max_q_len > paged_ops.MAX_TREE_NODES:
             raise ValueError(f"a tree of {self.max_q_len} nodes; at most {paged_ops.MAX_TREE_NODES}")
         paged_ops._require_device(cache.k)
-        self.tokens = [list(t) for t in tokens]
+        self.tokens, self._trees = [list(t) for t in tokens], [list(t) for t in parents]
         self.starts = [cache.lengths[s] for s in self.slots]
         ends = [a + n for a, n in zip(self.starts, self.lengths)]
         s_n, n, nb = len(self.slots), sum(self.lengths), max(1, cache.blocks_for(max(ends)))
@@ -719,6 +719,8 @@ class PagedTreeContext:
         for s, end in zip(self.slots, ends):
             cache.ensure_capacity(s, end)
         cache.prepare_writes(self.slots, self.starts, self.lengths)
+        # Each sequence's table as the nodes are appended by it: the list itself and what it holds now.
+        self._held = [(cache.block_tables[s], list(cache.block_tables[s])) for s in self.slots]
         dev = cache.k.device
         # One upload: tokens (int64) | row offsets | cached lengths | parents | tables (int32).
         n32 = 2 * s_n + 1 + n + s_n * nb
@@ -784,16 +786,25 @@ class PagedTreeContext:
         return [[ids[i] for i in nodes[1:]] + [token] for ids, nodes, token in zip(self.tokens, kept, following.tolist())]
 
     def commit(self, path: torch.Tensor, counts: torch.Tensor) -> list[list[int]]:
-        """Keep the nodes ``path[s, :counts[s]]`` (node 0 first, each below a node before it): their rows are moved to
-        consecutive places and the sequences' lengths updated. Returns the paths. Once per step."""
+        """Keep the nodes ``path[s, :counts[s]]`` (node 0 first, each a child of the node before it): their rows are moved
+        to consecutive places and the sequences' lengths updated. Returns the paths. Once per step, and before anything
+        else is written to its sequences."""
         if self._settled:
             raise RuntimeError("this step's tokens have been committed")
-        nodes = [row[:k] for row, k in zip(path.tolist(), counts.tolist())]
-        if len(nodes) != len(self.slots):
-            raise ValueError(f"{len(nodes)} paths for {len(self.slots)} sequences")
-        for kept, n in zip(nodes, self.lengths):
-            if not kept or kept[0] != 0 or any(a >= b for a, b in zip(kept, kept[1:])) or kept[-1] >= n:
-                raise ValueError(f"not a path of nodes below {n} from the root on: {kept}")
+        rows, sizes = path.tolist(), counts.tolist()
+        if not len(rows) == len(sizes) == len(self.slots):
+            raise ValueError(f"{len(rows)} paths for {len(self.slots)} sequences, {len(sizes)} counts")
+        nodes = []
+        for row, k, tree in zip(rows, sizes, self._trees):
+            kept = row[:max(k, 0)]
+            if not kept or len(kept) != k or kept[0] != 0 or any(
+                    not a < b < len(tree) or tree[b] != a for a, b in zip(kept, kept[1:])):
+                raise ValueError(f"not a path of nodes below {len(tree)} from the root on: {kept} (count {k})")
+            nodes.append(kept)
+        for slot, start, (table, held) in zip(self.slots, self.starts, self._held):
+            if (self.cache.lengths.get(slot) != start or self.cache.block_tables[slot] is not table
+                    or table[:len(held)] != held):
+                raise RuntimeError(f"sequence {slot} has changed since this step was made")
         if any(kept[-1] != len(kept) - 1 for kept in nodes):  # else every row is in place
             paged_ops.tree_commit(self.cache.k, self.cache.v, self.block_tables, self.ctx_start, path, counts)
         self._settled = True

@@ -94,3 +94,91 @@ def test_a_token_that_no_index_holds_takes_no_blocks(host):
     with pytest.raises(OverflowError):
         cache.tree_context([a], [[1, 1 << 70]], [[-1, 0]])
     assert state(cache) == before
+
+
+I32 = dict(dtype=torch.int32)
+#      0
+#    1   2
+#   3   4 5
+TREE = [1, 2, 3, 4, 5, 6], [-1, 0, 0, 1, 2, 2]
+
+
+def tree_step(cache):
+    slot = sequence(cache, 6)
+    return slot, cache.tree_context([slot], [TREE[0]], [TREE[1]])
+
+
+@pytest.mark.parametrize("path,count", [
+    ([0, 1, 2], 3),      # two siblings
+    ([0, 3], 2),         # a node without its parent
+    ([0, 1, 4], 3),      # a child of another branch
+    ([0, 2, 5], -1),     # no such count
+    ([0, 2, 5], 4),      # more nodes than the path has
+    ([0, 2, 5], 0), ([0, 2, 6], 3), ([0, 0], 2), ([2, 5], 2), ([0, -1], 2)])
+def test_what_is_not_a_path_is_not_committed(host, path, count):
+    cache = make_cache(num_blocks=8)
+    slot, ctx = tree_step(cache)
+    with pytest.raises(ValueError, match="not a path"):
+        ctx.commit(torch.tensor([path], **I32), torch.tensor([count], **I32))
+    assert cache.lengths[slot] == 6 and not host.moves
+    assert ctx.commit(torch.tensor([[0, 2, 5]], **I32), torch.tensor([3], **I32)) == [[0, 2, 5]]  # it can still be settled
+    assert cache.lengths[slot] == 9 and len(host.moves) == 1
+
+
+@pytest.mark.parametrize("path", [[0], [0, 1], [0, 2], [0, 1, 3], [0, 2, 4], [0, 2, 5]])
+def test_every_path_from_the_root_is_committed(host, path):
+    cache = make_cache(num_blocks=8)
+    slot, ctx = tree_step(cache)
+    padded = path + [-1] * (6 - len(path))
+    assert ctx.commit(torch.tensor([padded], **I32), torch.tensor([len(path)], **I32)) == [path]
+    assert cache.lengths[slot] == 6 + len(path)
+    assert len(host.moves) == (path not in ([0], [0, 1]))  # those lie in place
+
+
+def test_counts_and_paths_of_other_batches_are_refused(host):
+    cache = make_cache(num_blocks=8)
+    _, ctx = tree_step(cache)
+    for path, counts in (([[0], [0]], [1]), ([[0]], [1, 1]), ([[0], [0]], [1, 1])):
+        with pytest.raises(ValueError, match="paths for"):
+            ctx.commit(torch.tensor(path, **I32), torch.tensor(counts, **I32))
+
+
+def stale_length(cache, slot):
+    cache.ensure_capacity(slot, 7)
+    cache.lengths[slot] += 1
+
+
+def freed(cache, slot):
+    cache.free(slot)
+
+
+def reused(cache, slot):
+    cache.free(slot)
+    other = sequence(cache, 12)
+    assert sequence(cache, 6) == slot or other == slot
+    cache.lengths[slot] = 6
+
+
+def forked_and_written(cache, slot):
+    cache.fork(slot)
+    cache.prepare_writes([slot], [6], [2])
+
+
+@pytest.mark.parametrize("change", [stale_length, freed, reused, forked_and_written])
+def test_a_step_made_before_the_sequence_changed_is_not_committed(host, change):
+    """Its rows lie where the nodes were appended, which is not behind the sequence's tokens any more."""
+    cache = make_cache(num_blocks=8)
+    slot, ctx = tree_step(cache)
+    change(cache, slot)
+    before = state(cache)
+    with pytest.raises(RuntimeError, match="changed since"):
+        ctx.commit(torch.tensor([[0, 2, 5]], **I32), torch.tensor([3], **I32))
+    assert state(cache) == before and not host.moves
+
+
+def test_a_fork_made_before_the_commit_leaves_it_valid(host):
+    cache = make_cache(num_blocks=8)
+    slot, ctx = tree_step(cache)
+    child = cache.fork(slot)
+    assert ctx.commit(torch.tensor([[0, 2, 5]], **I32), torch.tensor([3], **I32)) == [[0, 2, 5]]
+    assert cache.lengths[slot] == 9 and cache.lengths[child] == 6
