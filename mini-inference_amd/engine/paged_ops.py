@@ -912,8 +912,8 @@ def paged_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
 class TreeStepCalls(PrefillStepCalls):
     """The layer calls of one step of drafted trees; the nodes are appended as a packed prefill's tokens are.
 
-    The calls of a step share one piece of scratch memory, which the first of them allocates: they belong on one stream,
-    or into one graph, in order, as a model issues them."""
+    Each call has scratch memory of its own, as :func:`paged_tree`'s do: layers may run on any stream, and in several
+    graphs."""
 
     def __init__(self, block_tables: torch.Tensor, cu_q: torch.Tensor, ctx_start: torch.Tensor, mask: torch.Tensor,
                  slot_mapping: torch.Tensor, max_q_len: int, scale: float) -> None:
@@ -925,11 +925,16 @@ class TreeStepCalls(PrefillStepCalls):
         key = (_layout(q), _layout(k_pool), _layout(v_pool))
         hit = self._hit("attend", key, layer)
         if hit is not None:
-            _, step, _, kb, vb, _, _ = hit
+            _, at, _, kb, vb, step, _ = hit
             _, hq, n, d = q.shape
             out = torch.empty_strided((1, hq, n, d), (hq * d, d, hq * d, 1), dtype=q.dtype, device=q.device)
+            if step.workspace_bytes:
+                # A copy of the struct, as another thread may be at a call of this step.
+                workspace = _scratch(None, q.device, step.workspace_bytes)
+                step = _native.TreeStep.from_buffer_copy(step)
+                step.workspace, at = workspace.data_ptr(), ctypes.addressof(step)
             _call_on(q.device, _native.load().mip_tree_step_attend,
-                     (step, out.data_ptr(), q.data_ptr(), k_pool.data_ptr() + layer * kb, v_pool.data_ptr() + layer * vb),
+                     (at, out.data_ptr(), q.data_ptr(), k_pool.data_ptr() + layer * kb, v_pool.data_ptr() + layer * vb),
                      "mip_tree_step_attend")
             return out
         q1 = q[0].transpose(0, 1)
@@ -938,10 +943,9 @@ class TreeStepCalls(PrefillStepCalls):
         if a is not None:
             _call_on(q.device, _native.load().mip_paged_tree, a, "mip_paged_tree")
             if q.shape[0] == 1:
-                step = _native.TreeStep(a[1], a[2], a[4], a[5], a[8], a[9], a[10], a[11], a[12], a[13], a[14], a[24], a[25],
+                step = _native.TreeStep(a[1], a[2], a[4], a[5], a[8], a[9], a[10], a[11], a[12], a[13], a[14], None, a[25],
                                         *a[15:23], a[26], a[23])
-                self._keep("attend", key, step, k_pool, v_pool, (self.block_tables, self.cu_q, self.ctx_start, self.mask,
-                                                                 workspace))
+                self._keep("attend", key, step, k_pool, v_pool, (self.block_tables, self.cu_q, self.ctx_start, self.mask))
         return out.transpose(0, 1).unsqueeze(0)
 
 

@@ -108,3 +108,47 @@ def test_a_prefill_context_follows_what_is_assigned_to_it(library):
         kept = ctx.calls
     ctx.write_at = (offsets, blocks)
     assert ctx.write_at[0] is offsets and ctx.write_at[1] is blocks
+
+
+def test_every_layer_of_a_tree_step_has_scratch_memory_of_its_own(library, monkeypatch):
+    """Layer calls that may run at once (two streams, a graph and eager calls) do not meet in one workspace: each takes
+    memory from its own stream's allocator, which no call holds on to."""
+    from engine import _native, paged_ops
+
+    taken, at_launch = [], []
+    empty = torch.empty
+
+    def noted(*size, **kw):
+        t = empty(*size, **kw)
+        if kw.get("dtype") is torch.uint8:
+            taken.append(t)
+        return t
+
+    def call(fn, args):
+        if fn == "mip_tree_step_attend":
+            step = _native.TreeStep.from_address(args[0])
+            at_launch.append((step.workspace, step.workspace_bytes))
+        else:
+            at_launch.append((args[24], args[25]))
+        return 0
+
+    for name in ("mip_paged_tree", "mip_tree_step_attend"):
+        monkeypatch.setattr(library, name, lambda *args, name=name: call(name, args), raising=False)
+    monkeypatch.setattr(paged_ops, "_one_device", lambda *tensors: tensors[0].device)
+    monkeypatch.setattr(paged_ops, "_call_on", lambda device, fn, args, what: fn(*args, 0))
+    monkeypatch.setattr(paged_ops, "_tree_bytes", lambda *shape: 4096)
+    monkeypatch.setattr(torch, "empty", noted)
+    k_pool, v_pool = torch.zeros(4, 9, 2, 16, 16), torch.zeros(4, 9, 2, 16, 16)
+    cu = torch.tensor([0, 5, 8], dtype=torch.int32)
+    calls = paged_ops.TreeStepCalls(torch.arange(4, dtype=torch.int32).view(2, 2), cu, torch.tensor([3, 1], dtype=torch.int32),
+                                    torch.ones(8, 1, dtype=torch.int64), torch.arange(8), 5, 0.25)
+    for layer in range(4):
+        q, _, _ = _qkv(1, 8)
+        calls.attend(layer, q, k_pool, v_pool)
+    assert len(at_launch) == len(taken) == 4
+    assert [a for a, _ in at_launch] == [t.data_ptr() for t in taken] and len({a for a, _ in at_launch}) == 4
+    assert {n for _, n in at_launch} == {4096}
+    refs = [StorageWeakRef(t.untyped_storage()) for t in taken]
+    taken.clear()
+    gc.collect()
+    assert all(r.expired() for r in refs)
