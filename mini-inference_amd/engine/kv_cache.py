@@ -513,7 +513,7 @@ class PagedDecodeContext:
 
 
 def _step_input(name: str) -> property:
-    """An attribute that a prefill context's layer calls are laid out for: assigning it has them laid out again."""
+    """An attribute that a context's layer calls are laid out for: assigning it has them laid out again."""
 
     def put(self, value) -> None:
         setattr(self, "_" + name, value)
@@ -682,6 +682,8 @@ class PagedTreeContext:
     """
 
     fuse_rope = True
+    block_tables, cu_q, ctx_start, mask, slot_mapping, max_q_len = map(
+        _step_input, ("block_tables", "cu_q", "ctx_start", "mask", "slot_mapping", "max_q_len"))
 
     def __init__(self, cache: PagedKVCache, slots: Sequence[int], tokens: Sequence[Sequence[int]],
                  parents: Sequence[Sequence[int]]) -> None:

@@ -182,3 +182,19 @@ def test_a_fork_made_before_the_commit_leaves_it_valid(host):
     child = cache.fork(slot)
     assert ctx.commit(torch.tensor([[0, 2, 5]], **I32), torch.tensor([3], **I32)) == [[0, 2, 5]]
     assert cache.lengths[slot] == 9 and cache.lengths[child] == 6
+
+
+def test_a_tree_context_follows_what_is_assigned_to_it(host):
+    """A mask, tables or slots put in the place of the step's own reach the layer calls, also after the first of them."""
+    cache = make_cache(num_blocks=8)
+    _, ctx = tree_step(cache)
+    kept = ctx.calls
+    assert ctx.calls is kept
+    ctx.other = 1
+    assert ctx.calls is kept
+    for name in ("block_tables", "cu_q", "ctx_start", "mask", "slot_mapping"):
+        setattr(ctx, name, getattr(ctx, name).clone())
+        assert ctx.calls is not kept and getattr(ctx.calls, name) is getattr(ctx, name), name
+        kept = ctx.calls
+    ctx.max_q_len = 7
+    assert ctx.calls.max_q_len == 7
