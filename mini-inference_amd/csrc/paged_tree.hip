@@ -1088,8 +1088,9 @@ __global__ __launch_bounds__(256) void paged_tree_row_kernel(TreeArgs a, PartArg
       for (int e = 0; e < N; ++e) dot = fmaf(qf[e], widen<DT>(kr[e]), dot);
 #pragma unroll
       for (int o = 1; o < LPR; o <<= 1) dot += __shfl_xor(dot, o);
-      if (!seen[u] || dot == -INFINITY) continue;
-      const float sc = dot * a.scale_log2, mn = fmax2(m, sc);
+      const float sc = dot * a.scale_log2;  // -inf also where a finite product's score is below fp32: it weighs nothing
+      if (!seen[u] || sc == -INFINITY) continue;
+      const float mn = fmax2(m, sc);
       const float alpha = fast_exp2(m - mn), pk = fast_exp2(sc - mn);  // m = -inf before any key: alpha 0
       l = l * alpha + pk;
 #pragma unroll

@@ -1,0 +1,60 @@
+"""Drafted-tree attention where rounding or the range of fp32 shows, against the plain 64-bit form.
+
+Bound of an output element (see test_gpu_tree.py for the scores): a weight is off by a relative
+delta = (D + 2) 2^-24 reach + 2^-21 (score, exp2) and, on the 16-bit matrix cores, by what is left of it beside its two
+16-bit parts: a part rounds to half a step h (fp16 2^-11, bf16 2^-8), so two leave h^2 of it at most, fp16 parts 2^-32
+of the row's largest weight besides. Weights enter the sum and the normaliser; fp32 sums over n keys add n 2^-23. Times
+the weighted mean of |v|, and half a step of the output on top, nothing absolute.
+"""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from conftest import announce
+from test_gpu_tree import DTYPES, Step, run, widened
+
+pytestmark = pytest.mark.gpu
+
+
+def bound_of(step, out, spread, reach, keys):
+    half_step = torch.finfo(DTYPES[step.dtype]).eps / 2
+    delta = (step.d + 2) * 2.0**-24 * reach + 2.0**-21 + keys * 2.0**-23
+    if step.dtype != "float32":
+        delta = delta + half_step**2 + keys * 2.0**-32
+    least = torch.finfo(DTYPES[step.dtype]).smallest_normal * half_step
+    return 1.01 * half_step * np.abs(out) + 2.05 * delta[..., None] * spread + least
+
+
+def wide(step, gpu, large):
+    """The call's arguments; large False: as they are, None: with tables of 2000 tokens, at which the matrix cores are taken
+    for short contexts too, True: with tables at which a call of more than 64 rows is a large one."""
+    args = step.to(gpu)
+    if large is None:
+        tab = torch.full((len(step.nodes), max(2000 // step.bs, step.width())), -1, dtype=torch.int32, device=gpu)
+        tab[:, :args["block_tables"].shape[1]] = args["block_tables"]
+        return {**args, "block_tables": tab}
+    return widened(step, args) if large else args
+
+
+@pytest.mark.parametrize("dtype,d,hq,hkv,bs,nodes,large", [
+    ("float32", 32, 4, 2, 16, [3], False), ("bfloat16", 32, 4, 2, 16, [3], False), ("float16", 256, 2, 1, 16, [3], False),
+    ("bfloat16", 64, 4, 2, 16, [3], False), ("float32", 64, 4, 2, 16, [3], False), ("float32", 128, 28, 4, 16, [30], False),
+    ("float16", 64, 14, 2, 16, [9], None), ("bfloat16", 128, 28, 4, 16, [40], None), ("bfloat16", 64, 14, 2, 16, [40], True), ("bfloat16", 128, 28, 4, 16, [40], True)])
+def test_scores_below_fp32_weigh_nothing(gpu, dtype, d, hq, hkv, bs, nodes, large):
+    """A product within fp32 whose score passes its range: -inf, in the first keys that are met and among later ones."""
+    announce(f"paged_tree scores below fp32 {dtype} d={d} nodes={nodes} large={large}")
+    step = Step(dtype, d, hq, hkv, bs, [150], nodes, seed=41, kind="free", scale=2.0**125)
+    step.qkv.zero_()
+    step.qkv[:, 0:hq * d:d] = 1.0
+    step.k.zero_()
+    for key in [*range(64), 70, 99, 140]:
+        step.k[step.tables[0][key // bs], :, key % bs, 0] = -16.0  # score -2^129
+    got = run(gpu, step, **wide(step, gpu, large)).double().cpu().numpy()
+    out, spread, reach = step.want()
+    assert np.isfinite(got).all()
+    assert (np.abs(got - out) <= bound_of(step, out, spread, 0 * reach, 200)).all()  # the seen scores are 0, exactly
