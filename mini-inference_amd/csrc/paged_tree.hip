@@ -36,13 +36,11 @@
 // 32000 keys 63 -> 104: four wavefronts wait at a barrier for loads that registers would have held back.)
 //
 // Roundings. Scores, sums and accumulators are fp32. fp16 V: the weights enter the product as fp16 (2^-11
-// relative; the sums are taken of the rounded weights, so the error of a lone key cancels). bf16 V with
-// own keys: V as it is, weights as a bf16 value and its remainder (2^-16); with shared keys V is staged
-// as fp16, once for all rows (exact from 2^-17 to 65280; one product instead of two: 65.1 -> 59.7 us and
-// 71.5 -> 63.5 on the two cases above), and a piece in which some dim's means are so small that this could
-// show runs again with V as it is. A wavefront whose accumulators end up inf or NaN does its part of a
-// piece again in a careful pass, which adds each value to the rows that see its key alone: a masked key
-// must not reach a row as 0 * inf.
+// relative; the sums are taken of the rounded weights, so the error of a lone key cancels). bf16 V: as it is, weights as
+// a bf16 value and its remainder (2^-16 of a weight is lost at most). (V staged as fp16 for one product instead of two
+// loses what lies below 2^-24, a row of small values beside ordinary ones entirely.) A wavefront whose accumulators end
+// up inf or NaN does its part of a piece again in a careful pass, which adds each value to the rows that see its key
+// alone: a masked key must not reach a row as 0 * inf.
 //
 // Measured (graph replay, us a call, both kernels): 128 sequences of 4-8 nodes, 28q/4kv d128, 512-8192
 // keys: 171, 725 MB at 4.2 TB/s; 64 x 33-64 nodes, 14q/2kv d64, 128-4096 keys: 50, 234 TFLOP/s; 61 nodes over
@@ -111,15 +109,6 @@ __device__ __forceinline__ uint2 lds_tr16(const char* p) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lv4_t*)(p)));
 }
 
-// Eight bf16 values -> fp16: exact from 2^-17 to 65280 in magnitude, inf from 65536 on; smaller ones land
-// on fp16's subnormal grid (a change of at most 2^-25).
-__device__ __forceinline__ u32x4_t bf16x8_to_f16x8(const u32x4_t& v) {
-  auto cv = [](uint32_t x) __attribute__((always_inline)) {
-    return MfmaOps<MIP_F16>::pack2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
-  };
-  return u32x4_t{cv(v[0]), cv(v[1]), cv(v[2]), cv(v[3])};
-}
-
 template <int D, int WR, int WK, int NC>
 struct Shape {
   static constexpr int NW = WR * WK;               // wavefronts
@@ -160,7 +149,6 @@ struct Shared {
   int start[kMaxSeqs];  // first step of every sequence's segments
   int cu[kMaxSeqs + 1], ctx[kMaxSeqs];
   uint32_t ok[2];       // byte w: every key that wavefront w copied exists and lies in a block of the pool
-  uint32_t redo;        // byte w: wavefront w found sums that need V as it is
 };
 
 // Node of query row r (group 1 has no 32-bit reciprocal).
@@ -232,43 +220,6 @@ struct Rows {
                     fmax2(fabsf(acc[c][mt][2]), fabsf(acc[c][mt][3])));
     // On the bits: the compiler takes a maximum of absolute values for a number and compares it as one.
     return __all(__float_as_uint(big) < 0x7f800000u);
-  }
-  // Of the whole wavefront: whether in some dim every row's weighted mean is below 2^-16, where the rounding of V to
-  // fp16's subnormal grid (2^-25) would show beside the rounding of the output. First within each lane's rows, which
-  // settles nearly every piece; then over the lanes.
-  __device__ __forceinline__ bool tiny() const {
-    constexpr float kSmall = 0x1p-16f;
-    f32x4_t top[MT];
-    bool some = false;
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const bool counts = live[c] && l[c][0] != 0.0f;
-      const float inv = counts ? __builtin_amdgcn_rcpf(l[c][0]) : 0.0f;
-      some = some || counts;
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x = fabsf(acc[c][mt][i] * inv);
-          top[mt][i] = c ? fmax2(top[mt][i], x) : x;
-        }
-    }
-    auto least = [&] {
-      float low = INFINITY;
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) low = top[mt][i] < low ? top[mt][i] : low;
-      return low;
-    };
-    if (!__any(some && least() < kSmall)) return false;  // (a NaN is not small)
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1)
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top[mt][i] = fmax2(top[mt][i], __shfl_xor(top[mt][i], o));
-    return __any(least() < kSmall);
   }
 };
 
@@ -344,14 +295,14 @@ template <class Ops> __device__ __forceinline__ uint4 pack8(const float (&x)[8])
 }
 
 // The weights' products with V^T and their sums. vt: lane (dim 16 mt + lane % 16): k index 8 grp + i stands for key
-// 4 grp + i (i < 4) or 16 + 4 grp + i - 4, the keys of this lane's scores, so the weights stay where they are. VT: the
-// type of V in vt. Weights enter as VT, for bf16 with their rounding remainders as a second product.
-template <int VT, int D, int NC>
+// 4 grp + i (i < 4) or 16 + 4 grp + i - 4, the keys of this lane's scores, so the weights stay where they are.
+// They enter in V's type, for bf16 with their rounding remainders as a second product.
+template <int DT, int D, int NC>
 __device__ __forceinline__ void value_tile(Rows<D, NC>& rows, const u32x4_t (&vt)[D / 16], const float (&sv)[NC][8],
                                            float scale_log2) {
   constexpr int MT = D / 16;
-  using Ops = MfmaOps<VT>;
-  constexpr uint32_t kOne2 = VT == MIP_BF16 ? 0x3f803f80u : 0x3c003c00u;
+  using Ops = MfmaOps<DT>;
+  constexpr uint32_t kOne2 = DT == MIP_BF16 ? 0x3f803f80u : 0x3c003c00u;
   const uint4 ones = make_uint4(kOne2, kOne2, kOne2, kOne2);
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
@@ -361,7 +312,7 @@ __device__ __forceinline__ void value_tile(Rows<D, NC>& rows, const u32x4_t (&vt
     rows.l[c] = Ops::qk(ones, ph, rows.l[c]);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) rows.acc[c][mt] = Ops::qk(u4(vt[mt]), ph, rows.acc[c][mt]);
-    if constexpr (VT == MIP_BF16) {
+    if constexpr (DT == MIP_BF16) {
       const uint32_t h[4] = {ph.x, ph.y, ph.z, ph.w};
 #pragma unroll
       for (int i = 0; i < 8; ++i) pr[i] -= i & 1 ? Ops::hi(h[i / 2]) : Ops::lo(h[i / 2]);
@@ -601,9 +552,8 @@ __device__ __forceinline__ void private_pass(const TreeArgs& a, const Piece& p, 
 }
 
 // A workgroup's keys of a piece, staged by all its threads for all its wavefronts: two LDS stages of a step, the
-// next step's rows in registers meanwhile. WR x WK wavefronts: WK take different 32 keys of a step. VT: the type in
-// which V is staged, fp16 (once for all rows) or its own.
-template <int DT, int VT, int D, int WR, int WK, int NCK, int NC>
+// next step's rows in registers meanwhile. WR x WK wavefronts: WK take different 32 keys of a step.
+template <int DT, int D, int WR, int WK, int NCK, int NC>
 __device__ __forceinline__ void shared_pass(const TreeArgs& a, const Piece& p, Rows<D, NC>& rows, char* smem, Shared& sh,
                                             int w, int lane) {
   using P = Shape<D, WR, WK, NCK>;
@@ -659,10 +609,8 @@ __device__ __forceinline__ void shared_pass(const TreeArgs& a, const Piece& p, R
 #pragma unroll
     for (int j = 0; j < NLD; ++j) {
       const int idx = tid + j * P::T, r = idx / CPR, c = idx % CPR;
-      u32x4_t vv = vbuf[j];
-      if constexpr (DT != VT) vv = bf16x8_to_f16x8(vv);
       *reinterpret_cast<u32x4_t*>(st + r * RB + ((c ^ (r & (CPR - 1))) * 16)) = kbuf[j];
-      *reinterpret_cast<u32x4_t*>(st + P::TILE + r * RB + ((c ^ vsw<D>(r)) * 16)) = vv;
+      *reinterpret_cast<u32x4_t*>(st + P::TILE + r * RB + ((c ^ vsw<D>(r)) * 16)) = vbuf[j];
     }
     if (lane == 0) reinterpret_cast<uint8_t*>(&sh.ok[stage])[w] = okbuf ? 1 : 0;
   };
@@ -706,7 +654,7 @@ __device__ __forceinline__ void shared_pass(const TreeArgs& a, const Piece& p, R
       }
       float sv[NC][8];
       score_tile<DT, D, NC>(a, p, rows, k, key0, real, grp, sv);
-      value_tile<VT, D, NC>(rows, vt, sv, a.scale_log2);
+      value_tile<DT, D, NC>(rows, vt, sv, a.scale_log2);
     }
     if (t + 1 < p.step1) stash(stage ^ 1);
     __syncthreads();
@@ -759,24 +707,7 @@ __device__ __forceinline__ void run_piece(const TreeArgs& a, const Piece& p, flo
   if constexpr (P::kPrivate) {
     private_pass<DT, D, NC>(a, p, rows, (lchar_t*)(smem + w * P::kRing), wk, lane);
   } else {
-    shared_pass<DT, MIP_F16, D, WR, WK, NCK, NC>(a, p, rows, smem, sh, w, lane);
-    if constexpr (DT == MIP_BF16) {  // the workgroup's keys again where they are too small for fp16
-      const bool redo = rows.tiny();
-      if (lane == 0) reinterpret_cast<uint8_t*>(&sh.redo)[w] = redo ? 1 : 0;
-      __syncthreads();
-      if (__builtin_amdgcn_readfirstlane(sh.redo) != 0) {
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {  // one column block at a time: few registers beside the others' sums
-          Rows<D, 1> one;
-          one.load(a, p, first + c * WR, 0, i16, grp);
-          shared_pass<DT, DT, D, WR, WK, NCK, 1>(a, p, one, smem, sh, w, lane);
-          rows.m[c] = one.m[0];
-          rows.l[c] = one.l[0];
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) rows.acc[c][mt] = one.acc[0][mt];
-        }
-      }
-    }
+    shared_pass<DT, D, WR, WK, NCK, NC>(a, p, rows, smem, sh, w, lane);
   }
   // A wavefront whose accumulators hold inf or NaN does its part again.
   if (!rows.finite()) careful_pass<DT, D, NC, P::KT>(a, p, rows, first, WR, wk, lane);

@@ -58,3 +58,62 @@ def test_scores_below_fp32_weigh_nothing(gpu, dtype, d, hq, hkv, bs, nodes, larg
     out, spread, reach = step.want()
     assert np.isfinite(got).all()
     assert (np.abs(got - out) <= bound_of(step, out, spread, 0 * reach, 200)).all()  # the seen scores are 0, exactly
+
+
+def cancelling(dtype, d, hq, hkv, bs, nodes, mean, keys=9, seed=42):
+    """Cached keys with scores of 0 to 1, and values whose weighted mean is about ``mean`` / 9 in every dim: what a weight is
+    off by shows in the output, whose own rounding is small. The nodes are seen by nobody."""
+    step = Step(dtype, d, hq, hkv, bs, [keys], nodes, seed=seed, kind="free", scale=1.0)
+    step.mask[:] = 0
+    step.qkv.zero_()
+    step.qkv[:, 0:hq * d:d] = 1.0
+    gen = torch.Generator().manual_seed(seed)
+    at = [(step.tables[0][p // bs], p % bs) for p in range(keys)]
+    for h in range(hkv):
+        score = torch.rand(keys, generator=gen).to(DTYPES[dtype])
+        w = torch.exp(score.double())
+        v = torch.randn(keys, d, generator=gen).to(DTYPES[dtype])
+        v[-1] = (-(w[:-1, None] * v[:-1].double()).sum(0) / w[-1] + mean).to(v.dtype)
+        for (b, o), s, row in zip(at, score, v):
+            step.k[b, h, o] = 0
+            step.k[b, h, o, 0] = s
+            step.v[b, h, o] = row
+    return step
+
+
+SIZES = [(64, 14, 2, 16, [2]), (64, 14, 2, 16, [4]), (64, 14, 2, 16, [9]), (64, 14, 2, 16, [40]), (128, 28, 4, 32, [2]),
+         (128, 28, 4, 32, [4]), (128, 28, 4, 32, [9]), (128, 28, 4, 32, [40])]
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16"])
+@pytest.mark.parametrize("large,mean", [(False, 0.0), (True, 0.0), (True, 0.02)])
+@pytest.mark.parametrize("d,hq,hkv,bs,nodes", SIZES)
+def test_weights_keep_their_bits(gpu, dtype, large, mean, d, hq, hkv, bs, nodes):
+    if large and max(nodes) * (hq // hkv) <= 64:
+        pytest.skip("large calls of more than 64 rows have a kernel of their own")
+    announce(f"paged_tree cancelling values {dtype} d={d} nodes={nodes} large={large}")
+    step = cancelling(dtype, d, hq, hkv, bs, nodes, mean)
+    got = run(gpu, step, **wide(step, gpu, large or None)).double().cpu().numpy()
+    out, spread, reach = step.want()
+    assert np.abs(out).max() < 0.02 * spread.max()
+    err, bound = np.abs(got - out), bound_of(step, out, spread, reach, 9)
+    assert (err <= bound).all(), float((err / bound).max())
+
+
+@pytest.mark.parametrize("d,hq,hkv", [(64, 14, 2), (128, 28, 4)])
+@pytest.mark.parametrize("small", [2.0**-19, 2.0**-26, 2.0**-60])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_a_row_of_small_values_beside_ordinary_ones(gpu, d, hq, hkv, small, zeros):
+    """Nothing cached: a root that sees itself alone, a node that sees it and another small one; with and without a dim of zeros."""
+    announce(f"paged_tree large call, one row of {small} d={d}")
+    step = Step("bfloat16", d, hq, hkv, 16, [0, 31], [40, 12], seed=43, kind="free")
+    step.mask[0], step.mask[7] = 1, (1 << 7) | 1
+    for node in (0, 7):
+        step.v[step.tables[0][node // 16], :, node % 16] *= small
+    if zeros:
+        step.v[..., 5] = 0
+    got = run(gpu, step, **wide(step, gpu, True)).double().cpu().numpy()
+    out, spread, reach = step.want()
+    err, bound = np.abs(got - out), bound_of(step, out, spread, reach, 52)
+    assert (err <= bound).all(), float((err / bound).max())
+    assert np.abs(got[[0, 7]]).max() > 0 and (got[..., 5] == 0).all() == zeros
