@@ -443,8 +443,8 @@ int mip_rope_tables(void* cos, void* sin, const int64_t* positions, int32_t n_to
  * bytes are, and a key whose block id lies outside the pool is seen by no row. Keys past
  * max_blocks_per_seq * block_size are never read. mask_words >= ceil(max_q_len / 64). scale > 0.
  * Scores, sums and products accumulate in fp32; 16-bit types at head_dim 64 / 128 (q rows 16-byte, output
- * rows 8-byte aligned) run on the matrix cores, with the softmax weights rounded to fp16 as in mip_paged_prefill (fp16
- * calls) or as a bf16 value and its remainder (bf16 calls, whose values are multiplied as they are); fp32 at these
+ * rows 8-byte aligned) run on the matrix cores, with the softmax weights as a 16-bit value and its remainder (off by
+ * 2^-22 in fp16, 2^-16 in bf16 at most) and the cached values as they are; fp32 at these
  * head sizes runs on the fp32 matrix cores. Short calls of few rows, and all others, take a workgroup per (node,
  * query head): any type, head_dim a power of two in 8 .. 256 (others: MIP_EUNSUPPORTED), element alignment.
  * Nodes from max_q_len on are neither rows nor keys. out must not overlap the inputs.

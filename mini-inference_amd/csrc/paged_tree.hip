@@ -35,9 +35,10 @@
 // (Direct loads for the shared shape were slower: 64 x 33-64 nodes of 7 rows 58 -> 66 us, one of 61 nodes over
 // 32000 keys 63 -> 104: four wavefronts wait at a barrier for loads that registers would have held back.)
 //
-// Roundings. Scores, sums and accumulators are fp32. fp16 V: the weights enter the product as fp16 (2^-11
-// relative; the sums are taken of the rounded weights, so the error of a lone key cancels). bf16 V: as it is, weights as
-// a bf16 value and its remainder (2^-16 of a weight is lost at most). (V staged as fp16 for one product instead of two
+// Roundings. Scores, sums and accumulators are fp32. Weights enter the product in V's type, as a 16-bit value and its
+// remainder: 2^-22 of a weight is lost at most in fp16 (and 2^-32 of a row's largest), 2^-16 in bf16. (The value alone,
+// one product instead of two: 64 x 33-64 nodes in fp16 49.7 us instead of 55.0, but weights off by 2^-11, which shows
+// wherever values nearly cancel.) V enters as it is. (V staged as fp16 for one product instead of two
 // loses what lies below 2^-24, a row of small values beside ordinary ones entirely.) A wavefront whose accumulators end
 // up inf or NaN does its part of a piece again in a careful pass, which adds each value to the rows that see its key
 // alone: a masked key must not reach a row as 0 * inf.
@@ -296,7 +297,7 @@ template <class Ops> __device__ __forceinline__ uint4 pack8(const float (&x)[8])
 
 // The weights' products with V^T and their sums. vt: lane (dim 16 mt + lane % 16): k index 8 grp + i stands for key
 // 4 grp + i (i < 4) or 16 + 4 grp + i - 4, the keys of this lane's scores, so the weights stay where they are.
-// They enter in V's type, for bf16 with their rounding remainders as a second product.
+// They enter in V's type, with their rounding remainders as a second product.
 template <int DT, int D, int NC>
 __device__ __forceinline__ void value_tile(Rows<D, NC>& rows, const u32x4_t (&vt)[D / 16], const float (&sv)[NC][8],
                                            float scale_log2) {
@@ -312,15 +313,13 @@ __device__ __forceinline__ void value_tile(Rows<D, NC>& rows, const u32x4_t (&vt
     rows.l[c] = Ops::qk(ones, ph, rows.l[c]);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) rows.acc[c][mt] = Ops::qk(u4(vt[mt]), ph, rows.acc[c][mt]);
-    if constexpr (DT == MIP_BF16) {
-      const uint32_t h[4] = {ph.x, ph.y, ph.z, ph.w};
+    const uint32_t h[4] = {ph.x, ph.y, ph.z, ph.w};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) pr[i] -= i & 1 ? Ops::hi(h[i / 2]) : Ops::lo(h[i / 2]);
-      const uint4 pl = pack8<Ops>(pr);
-      rows.l[c] = Ops::qk(ones, pl, rows.l[c]);
+    for (int i = 0; i < 8; ++i) pr[i] -= i & 1 ? Ops::hi(h[i / 2]) : Ops::lo(h[i / 2]);
+    const uint4 pl = pack8<Ops>(pr);
+    rows.l[c] = Ops::qk(ones, pl, rows.l[c]);
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) rows.acc[c][mt] = Ops::qk(u4(vt[mt]), pl, rows.acc[c][mt]);
-    }
+    for (int mt = 0; mt < MT; ++mt) rows.acc[c][mt] = Ops::qk(u4(vt[mt]), pl, rows.acc[c][mt]);
   }
 }
 

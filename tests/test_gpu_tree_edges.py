@@ -85,7 +85,7 @@ SIZES = [(64, 14, 2, 16, [2]), (64, 14, 2, 16, [4]), (64, 14, 2, 16, [9]), (64, 
          (128, 28, 4, 32, [4]), (128, 28, 4, 32, [9]), (128, 28, 4, 32, [40])]
 
 
-@pytest.mark.parametrize("dtype", ["bfloat16"])
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
 @pytest.mark.parametrize("large,mean", [(False, 0.0), (True, 0.0), (True, 0.02)])
 @pytest.mark.parametrize("d,hq,hkv,bs,nodes", SIZES)
 def test_weights_keep_their_bits(gpu, dtype, large, mean, d, hq, hkv, bs, nodes):
