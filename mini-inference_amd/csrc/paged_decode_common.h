@@ -49,7 +49,7 @@ struct DecodeArgs {
 
 // Drafted trees: node i of sequence s (packed row cu_q[s] + i) sees its sequence's ctx_start[s] cached keys and the
 // nodes e whose bits are set in its row of the mask. Key ranges of part_tokens keys: blockIdx.z of the grid, records
-// as for decode partitions with the packed row as the sequence.
+// as for decode partitions with row s * max_q_len + i as the sequence (not the packed row: trees differ in size).
 struct TreeMask {
   const uint64_t* mask;
   int64_t stride;  // words

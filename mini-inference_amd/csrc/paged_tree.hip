@@ -871,6 +871,7 @@ __global__ __launch_bounds__(256) void paged_tree_merge(TreeArgs a, int segs_per
   const int lane = threadIdx.x & (kWave - 1), i16 = lane & 15, w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int s = blockIdx.x / segs_per_seq, seg = blockIdx.x - s * segs_per_seq;
   const int cb = BY_PIECE ? blockIdx.y : blockIdx.y * 4 + w;
+  if (cb >= R / 16) return;  // shapes of fewer than four column blocks (whole wavefronts; BY_PIECE has none such)
   Piece p;
   p.s = s;
   p.q = seq_of(a, s);
