@@ -481,6 +481,7 @@ int mip_tree_index(int64_t* positions, int64_t* slot_mapping, uint64_t* mask, in
  *     target[r]     = the lowest index of row r's greatest logit (NaN counts as the greatest), all n_rows rows
  *     path[s]       = node 0, then from each node on to its lowest child (parents[r] = that node) whose
  *                     token tokens[r] is the node's target, until there is none; -1 from counts[s] on
+ *                     (of siblings that carry one token the first, whatever follows the others)
  *     next_token[s] = target of the path's last node (-1, with counts[s] = 0, for an empty tree)
  * path has max_q_len entries a sequence; max_q_len at most MIP_TREE_MAX_NODES. The workspace holds
  * mip_tree_verify_workspace(..) bytes, 8-byte aligned.

@@ -1,11 +1,12 @@
 // Verification of drafted trees against a model's logits: the model's choice after every node, and the
-// longest drafted path that agrees with it.
+// drafted path that agrees with it, at every node its first child that does.
 //
 // No reference counterpart (the reference decodes one token a step). For row r of the logits
 //     target[r] = the lowest v with logits[r][v] = max (a NaN counts as the greatest value)
 // and for sequence s, whose tree's node i is row cu_q[s] + i, the path starts at node 0 and goes on to the
 // lowest node whose parent is the path's last node and whose token is that node's target, until there is
-// none; the target of the last node is the token that follows.
+// none; the target of the last node is the token that follows. (Of siblings that carry one token the first is
+// taken, whatever is drafted below the others.)
 //
 // Two launches. verify_max: a workgroup takes a piece of a row (rows are cut where there are few of them)
 // and leaves its maximum as one 64-bit key, (value in an order-preserving integer form) << 32 |

@@ -777,11 +777,12 @@ class PagedTreeContext:
         return paged_ops.tree_verify(logits, self.input_ids, self.parents, self.cu_q, self.max_q_len)
 
     def accept(self, logits: torch.Tensor) -> list[list[int]]:
-        """Greedy verification: keep the longest path that the logits agree with; returns each sequence's new tokens.
+        """Greedy verification: keep the path that the logits agree with; returns each sequence's new tokens.
 
-        Those are the path's drafted tokens and the model's token after them (one at least: what a decode step
-        would have returned). The root and the path's tokens are cached and counted from then on; the last new
-        token is not, and is the next step's root.
+        Of siblings that carry the agreed token the first is taken, whatever is drafted below the others: a draft's
+        equal continuations belong under one node. The new tokens are the path's drafted tokens and the model's token
+        after them (one at least: what a decode step would have returned). The root and the path's tokens are cached
+        and counted from then on; the last new token is not, and is the next step's root.
         """
         _, path, counts, following = self.verify(logits)
         kept = self.commit(path, counts)

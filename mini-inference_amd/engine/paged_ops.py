@@ -965,7 +965,8 @@ def tree_verify(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
     ``logits`` ``[N, vocab]`` (rows contiguous): the model's answer after every node; ``tokens`` int64 ``[N]`` the
     nodes' tokens, ``parents`` and ``cu_q`` as for :func:`tree_index`. ``target`` (int64 ``[N]``): the lowest index
     of each row's greatest logit (a NaN counts as the greatest). ``path`` (int32 ``[S, max_q_len]``, -1 past the
-    end) starts at node 0 and goes on to the lowest child whose token is the last node's target, until there is none;
+    end) starts at node 0 and goes on to the lowest child whose token is the last node's target, until there is none (of
+    siblings that carry one token the first, whatever follows the others);
     ``counts`` (int32 ``[S]``) are the paths' lengths and ``next_token`` (int64 ``[S]``) the target of each one's last node
     (an empty tree: 0 and -1). Scratch memory as for :func:`paged_tree`.
     """

@@ -81,16 +81,13 @@ def cancelling(dtype, d, hq, hkv, bs, nodes, mean, keys=9, seed=42):
     return step
 
 
-SIZES = [(64, 14, 2, 16, [2]), (64, 14, 2, 16, [4]), (64, 14, 2, 16, [9]), (64, 14, 2, 16, [40]), (128, 28, 4, 32, [2]),
-         (128, 28, 4, 32, [4]), (128, 28, 4, 32, [9]), (128, 28, 4, 32, [40])]
+SIZES = [(d, hq, hkv, bs, [n], False, 0.0) for d, hq, hkv, bs in ((64, 14, 2, 16), (128, 28, 4, 32)) for n in (2, 4, 9, 40)]
+LARGE_SIZES = [(d, hq, hkv, bs, [40], True, mean) for d, hq, hkv, bs in ((64, 14, 2, 16), (128, 28, 4, 32)) for mean in (0.0, 0.02)]
 
 
 @pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
-@pytest.mark.parametrize("large,mean", [(False, 0.0), (True, 0.0), (True, 0.02)])
-@pytest.mark.parametrize("d,hq,hkv,bs,nodes", SIZES)
-def test_weights_keep_their_bits(gpu, dtype, large, mean, d, hq, hkv, bs, nodes):
-    if large and max(nodes) * (hq // hkv) <= 64:
-        pytest.skip("large calls of more than 64 rows have a kernel of their own")
+@pytest.mark.parametrize("d,hq,hkv,bs,nodes,large,mean", SIZES + LARGE_SIZES)
+def test_weights_keep_their_bits(gpu, dtype, d, hq, hkv, bs, nodes, large, mean):
     announce(f"paged_tree cancelling values {dtype} d={d} nodes={nodes} large={large}")
     step = cancelling(dtype, d, hq, hkv, bs, nodes, mean)
     got = run(gpu, step, **wide(step, gpu, large or None)).double().cpu().numpy()
@@ -117,3 +114,18 @@ def test_a_row_of_small_values_beside_ordinary_ones(gpu, d, hq, hkv, small, zero
     err, bound = np.abs(got - out), bound_of(step, out, spread, reach, 52)
     assert (err <= bound).all(), float((err / bound).max())
     assert np.abs(got[[0, 7]]).max() > 0 and (got[..., 5] == 0).all() == zeros
+
+
+def test_of_siblings_with_one_token_the_first_is_taken(gpu):
+    """Whatever follows the others, in kernel and plain form alike; the tokens are the greedy ones in any case."""
+    from oracle import tree_ref as ref
+    from test_gpu_tree import check_verify
+
+    announce("tree_verify equal siblings")
+    logits = np.full((6, 10), -1.0)
+    for r, t in enumerate([5, 7, 7, 2, 3, 0]):
+        logits[r, t] = 1.0
+    tokens, parents = [[1, 5, 5, 7, 7, 2]], [[-1, 0, 0, 2, 2, 3]]
+    _, paths, following = ref.verify(logits, tokens, parents)
+    assert paths == [[0, 1]] and following == [7]
+    check_verify(gpu, torch.from_numpy(logits).float().to(gpu), tokens, parents)
