@@ -721,8 +721,9 @@ class PagedTreeContext:
         for s, end in zip(self.slots, ends):
             cache.ensure_capacity(s, end)
         cache.prepare_writes(self.slots, self.starts, self.lengths)
-        # Each sequence's table as the nodes are appended by it: the list itself and what it holds now.
-        self._held = [(cache.block_tables[s], list(cache.block_tables[s])) for s in self.slots]
+        # Each sequence's table, from the first of its nodes' blocks on, and these blocks as the nodes are appended.
+        self._held = [(cache.block_tables[s], a // cache.block_size, cache.block_tables[s][a // cache.block_size:])
+                      for s, a in zip(self.slots, self.starts)]
         dev = cache.k.device
         # One upload: tokens (int64) | row offsets | cached lengths | parents | tables (int32).
         n32 = 2 * s_n + 1 + n + s_n * nb
@@ -804,9 +805,9 @@ class PagedTreeContext:
                     not a < b < len(tree) or tree[b] != a for a, b in zip(kept, kept[1:])):
                 raise ValueError(f"not a path of nodes below {len(tree)} from the root on: {kept} (count {k})")
             nodes.append(kept)
-        for slot, start, (table, held) in zip(self.slots, self.starts, self._held):
+        for slot, start, (table, first, held) in zip(self.slots, self.starts, self._held):
             if (self.cache.lengths.get(slot) != start or self.cache.block_tables[slot] is not table
-                    or table[:len(held)] != held):
+                    or table[first:first + len(held)] != held):
                 raise RuntimeError(f"sequence {slot} has changed since this step was made")
         if any(kept[-1] != len(kept) - 1 for kept in nodes):  # else every row is in place
             paged_ops.tree_commit(self.cache.k, self.cache.v, self.block_tables, self.ctx_start, path, counts)

@@ -129,3 +129,29 @@ def test_of_siblings_with_one_token_the_first_is_taken(gpu):
     _, paths, following = ref.verify(logits, tokens, parents)
     assert paths == [[0, 1]] and following == [7]
     check_verify(gpu, torch.from_numpy(logits).float().to(gpu), tokens, parents)
+
+
+@torch.inference_mode()
+def test_layer_calls_of_a_step_on_two_streams(gpu):
+    """A step's later layer calls, in flight on two streams at once, give what each gives alone (a long context, whose
+    pieces meet in scratch memory)."""
+    from engine.kv_cache import PagedKVCache
+
+    announce("tree layer calls on two streams")
+    cache = PagedKVCache(2, 2, 64, num_blocks=300, block_size=16, max_seqs=2, max_len=4600, dtype=torch.bfloat16, device=gpu)
+    slot = cache.allocate(4500)
+    cache.lengths[slot] = 4500
+    cache.k.normal_()
+    cache.v.normal_()
+    ctx = cache.tree_context([slot], [[1] * 9], [[-1, 0, 0, 1, 1, 2, 3, 4, 4]])
+    q = [torch.randn(1, 9, 14, 64, device=gpu).bfloat16().transpose(1, 2) for _ in range(2)]
+    want = [ctx.calls.attend(layer, q[layer], cache.k, cache.v) for layer in range(2)]
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    torch.cuda.synchronize()
+    for _ in range(6):
+        for layer, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append((layer, ctx.calls.attend(layer, q[layer], cache.k, cache.v)))
+    torch.cuda.synchronize()
+    for layer, out in got:
+        assert torch.equal(out, want[layer])
