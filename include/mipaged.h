@@ -441,7 +441,7 @@ int mip_rope_tables(void* cos, void* sin, const int64_t* positions, int32_t n_to
  *
  * A row that sees no key becomes zeros, a key that a row does not see has no influence on it whatever its
  * bytes are, and a key whose block id lies outside the pool is seen by no row. Keys past
- * max_blocks_per_seq * block_size are never read. mask_words >= ceil(max_q_len / 64). scale > 0.
+ * max_blocks_per_seq * block_size are never read. mask_words >= ceil(max_q_len / 64). 0 < scale <= 2^127.
  * Scores, sums and products accumulate in fp32; 16-bit types at head_dim 64 / 128 (q rows 16-byte, output
  * rows 8-byte aligned) run on the matrix cores, with the softmax weights as a 16-bit value and its remainder (off by
  * 2^-22 in fp16, 2^-16 in bf16 at most) and the cached values as they are; fp32 at these

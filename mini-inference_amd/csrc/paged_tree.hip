@@ -1273,7 +1273,8 @@ extern "C" int mip_paged_tree(void* out, int64_t out_stride_tok, int64_t out_str
   if (dtype != MIP_F32 && dtype != MIP_F16 && dtype != MIP_BF16) return MIP_EINVAL;
   if (num_seqs < 0 || max_q_len < 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads) return MIP_EINVAL;
   if (head_dim <= 0 || num_cache_blocks <= 0 || max_blocks_per_seq <= 0 || bt_stride < max_blocks_per_seq) return MIP_EINVAL;
-  if (!is_pow2(block_size) || block_size > 4096 || num_cache_blocks > INT32_MAX || !(scale > 0.0f)) return MIP_EINVAL;
+  if (!is_pow2(block_size) || block_size > 4096 || num_cache_blocks > INT32_MAX || !(scale > 0.0f && scale <= 0x1p127f))
+    return MIP_EINVAL;
   if (num_seqs == 0 || max_q_len == 0) return MIP_OK;
   if (!out || !q || !k_cache || !v_cache || !block_tables || !cu_q || !ctx_start || !mask) return MIP_EINVAL;
   if (mask_words < (max_q_len + 63) / 64 || mask_stride < mask_words) return MIP_EINVAL;

@@ -862,8 +862,8 @@ def _tree_args(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
             bits[1] > 1 and bit_strides[1] != 1):
         raise ValueError(f"mask must be int64 [{n}, >= {words}] with contiguous rows, got {tuple(bits)} {mask.dtype}")
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    if not 0.0 < scale < math.inf:
-        raise ValueError(f"scale={scale} must be positive")
+    if not 2.0**-149 <= scale <= 2.0**127:  # in base 2 it has to be an fp32 number
+        raise ValueError(f"scale={scale} must be positive and at most 2^127")
     if out is None:
         device = _one_device(q, k_cache, v_cache, block_tables, cu_q, ctx_start, mask)
         out, to = torch.empty_like(q, memory_format=torch.contiguous_format), (hq * d, d)
