@@ -44,8 +44,8 @@
 // alone: a masked key must not reach a row as 0 * inf.
 //
 // Measured (graph replay, us a call, both kernels): 128 sequences of 4-8 nodes, 28q/4kv d128, 512-8192
-// keys: 171, 725 MB at 4.2 TB/s; 64 x 33-64 nodes, 14q/2kv d64, 128-4096 keys: 50, 234 TFLOP/s; 61 nodes over
-// 32000 keys, 28q/4kv d128: 66, 422 TFLOP/s; 32 x 8-24 nodes, 128-1024 keys: 19; 5 nodes over 37 keys: 4.0.
+// keys: 170, 725 MB at 4.3 TB/s; 64 x 33-64 nodes, 14q/2kv d64, 128-4096 keys: 55, 215 TFLOP/s; 61 nodes over
+// 32000 keys, 28q/4kv d128: 70, 398 TFLOP/s; 32 x 8-24 nodes, 128-1024 keys: 20; 5 nodes over 37 keys: 4.0.
 #include "paged_decode_common.h"
 
 namespace mip {
@@ -1108,12 +1108,14 @@ Config config_of() {
 // The workgroup's shape by the most rows a segment's kv head can have, and the products of the call (sequences x kv
 // heads x rows x keys). Wavefronts with the same 16, 32 or 64 rows and keys of their own need no staging together and
 // cut a segment finely; wavefronts with rows of their own that share keys read each key a quarter as often. The
-// second takes blocks of 8 tokens or more and pays for more rows than 64 once the call is large (graph replay, us, own keys / shared; sequences x nodes of 7
-// rows; d64, 2 kv heads: 16 x 24 over 1024 keys 19.1/23.0, 64 x 48 over 256 21.9/29.1, 64 x 24 over 1024 (22M) 28.6/30.8,
-// 64 x 32 over 1024 (29M) 36.7/32.5, 64 x 48 over 1024 43.2/37.9, 64 x 64 over 4096 109/84.7; d128, 4 kv heads: 4 x 24
-// over 4096 28.7/32.6, 1 x 16 over 32768 (15M) 33.4/34.8, 16 x 48 over 1024 (22M) 49.2/41.5, 16 x 64 over 4096 137/83.4).
-// d64 with shared keys: 32 rows a wavefront and three workgroups a CU against 64 and two, 64 x 64 over 512 36.0/39.0,
-// 256 x 64 over 512 66.9/73.2, 64 x 64 over 4096 87.0/85.8.
+// second takes blocks of 8 tokens or more and pays for more rows than 64 once the call is large (graph replay, us, own keys /
+// shared, bf16, fp16 the same within 4 %; sequences x half of to all of the nodes, of 7 rows each, over half of to all of
+// the keys; d64, 2 kv heads: 16 x 24 over 1024 keys 19.0/22.3, 64 x 48 over 256 21.8/27.7, 64 x 24 over 1024 (22M)
+// 30.3/29.7, 64 x 32 over 1024 (29M) 34.6/32.1, 64 x 48 over 1024 40.7/38.0, 64 x 64 over 4096 111/95.4; d128, 4 kv
+// heads: 4 x 24 over 4096 29.4/28.8, 1 x 16 over 32768 (15M) 33.2/30.6, 16 x 48 over 1024 (22M) 49.9/39.6, 16 x 64 over
+// 4096 139/93.3). The keys are the table's width: a call of short contexts with a wide table is taken for a large one.
+// d64 with shared keys: 32 rows a wavefront and three workgroups a CU against 64 and two, 64 x 64 over 512 35.5/38.9,
+// 256 x 64 over 512 71.9/81.8, 64 x 64 over 4096 95.0/100.
 template <int DT>
 Config pick(int d, int64_t rows, int64_t products, int bs) {
   if (d == 64) {
